@@ -459,6 +459,99 @@ mpp41_status mpp41_moe_ep(mpp41_ctx *ctx, const mpp41_moe_desc *desc, uint32_t c
                           const uint8_t *shared_sg, const uint8_t *shared_wu, const uint8_t *shared_su,
                           const uint8_t *shared_wd, const uint8_t *shared_sd, void *out, void *scratch);
 
+/* ---- expert routing with scores, a balance bias and groups (the router in front
+ *      of mpp41_moe_fp8; mpp41_moe_route is the plain top-k softmax; no reference
+ *      counterpart). Per token, over logits z [tokens][experts] (fp32, or fp16 with
+ *      logits_f16):
+ *        s = softmax(z) or sigmoid(z);  v = s + bias (bias [experts] fp32, or NULL).
+ *        A logit of -inf or NaN masks its expert: s = 0, v = -inf (a NaN sum too).
+ *        The experts form `groups` equal runs; a group's worth is the sum of its
+ *        group_top (1 or 2) largest v; the top_groups best groups stay.
+ *        ids[t][0..top_k) = the experts of those groups by falling v;
+ *        weights[t][j] = s of that expert, over the sum of the chosen with
+ *        renormalize (0 where that sum is 0: every chosen expert masked), times scale.
+ *      Ties go to the lower index, of experts and of groups. The choice does not
+ *      suffer from fp32 scores: without a bias (and without sums of two) it is made
+ *      on the logits, otherwise near ties are decided with scores in 64 bits. Masked experts are
+ *      chosen only where too few others are left, with weight 0.
+ *      experts <= 512; groups <= 32 divides experts; top_k <= 32 and at most
+ *      top_groups * experts / groups. ---- */
+enum { MPP41_GATE_SOFTMAX = 0, MPP41_GATE_SIGMOID = 1 };
+typedef struct {
+    uint32_t tokens, experts, top_k;
+    int32_t score;                            /* MPP41_GATE_* */
+    uint32_t groups, top_groups, group_top;   /* 1, 1, 1: no groups */
+    int32_t renormalize;
+    float scale;
+    int32_t logits_f16;
+} mpp41_gate_desc;
+mpp41_status mpp41_moe_gate(mpp41_ctx *ctx, const mpp41_gate_desc *desc, const void *logits, const float *bias,
+                            int32_t *ids, float *weights);
+
+/* ---- FP8 with an fp32 scale per block of 128 (no reference counterpart: its FP8
+ *      rows are unscaled). fmt: 1 = E4M3 (qmax 448), 2 = E5M2 (qmax 57344), as
+ *      mpp41_pack. value = q * scale.
+ *      - mpp41_quantize_act_fp8: fp16 x [tokens][hidden] -> q [tokens][hidden], scales
+ *        [tokens][ceil(hidden/128)]: per 1 x 128, scale = amax / qmax (1 where amax is
+ *        0), q = x * qmax / amax correctly rounded to nearest even. Infinities count
+ *        as +-65504; NaN stays NaN and does not enter amax.
+ *      - mpp41_quantize_weights_fp8: fp32 w [rows][depth] -> q [rows][depth], scales
+ *        [ceil(rows/128)][ceil(depth/128)]: per 128 x 128, scale = amax / qmax,
+ *        q = (w / amax) * qmax in fp32, rounded to nearest even. Infinities count as
+ *        the largest finite value.
+ *      Any sizes; buffers aligned to their elements (x 32-byte and q 16-byte aligned
+ *      with hidden % 16 == 0, or w 16-byte with depth % 4 == 0, runs wide accesses).
+ *      - mpp41_matmul_fp8: C[M][N] = A[M][K] B[N][K]^T, A with scales [M][ceil(K/128)],
+ *        B with scales [ceil(N/128)][ceil(K/128)], each operand of its own format; C
+ *        fp32 (c_f16 = 0) or fp16. Each block of 128 along K is summed on the tensor
+ *        cores and added up, scaled, in fp32.
+ *      - mpp41_matmul_fp8_grouped: rows [offsets[g], offsets[g+1]) of A and C with
+ *        B[g], B [groups][N][K], its scales [groups][ceil(N/128)][ceil(K/128)];
+ *        offsets [groups + 1] on the device, ascending within [0, M] (others are
+ *        clamped and reported as MPP41_ERR_BOUNDS by mpp41_synchronize). Rows of C
+ *        outside the groups are left as they are. groups <= 1024.
+ *      K a positive multiple of 16; M, groups * N and K below 2^31; A and B 16-byte
+ *      aligned. Results do not depend on the run: sums have a fixed order. ---- */
+mpp41_status mpp41_quantize_act_fp8(mpp41_ctx *ctx, int fmt, const void *x, uint32_t tokens, uint32_t hidden,
+                                    uint8_t *q, float *scales);
+mpp41_status mpp41_quantize_weights_fp8(mpp41_ctx *ctx, int fmt, const float *w, uint32_t rows, uint32_t depth,
+                                        uint8_t *q, float *scales);
+mpp41_status mpp41_matmul_fp8(mpp41_ctx *ctx, int a_fmt, const void *a, const float *sa, int b_fmt, const void *b,
+                              const float *sb, void *c, uint32_t M, uint32_t N, uint32_t K, int c_f16);
+mpp41_status mpp41_matmul_fp8_grouped(mpp41_ctx *ctx, int a_fmt, const void *a, const float *sa, int b_fmt,
+                                      const void *b, const float *sb, const int32_t *offsets, uint32_t groups, void *c,
+                                      uint32_t M, uint32_t N, uint32_t K, int c_f16);
+
+/* ---- expert layer in FP8 (W8A8 with the scales above), the routing given:
+ *        out[t] = shared_expert(x[t]) + sum_j weights[t][j] * expert_{ids[t][j]}(x[t])
+ *      over j < top_k in order; expert(x) = down(q(silu(gate(q(x))) * up(q(x)))) with
+ *      q the 1 x 128 activation quantizer (the mid in fp32 before it). A negative id
+ *      is no expert and adds nothing (a padded token, an expert of another rank); an
+ *      id of experts or more adds nothing either and is reported as
+ *      MPP41_ERR_BOUNDS by mpp41_synchronize. The same id twice in a token counts
+ *      twice. x fp16 [tokens][hidden], 32-byte aligned; ids and weights
+ *      [tokens][top_k] as mpp41_moe_gate writes them; weights of `fmt`: wg, wu
+ *      [experts][intermediate][hidden] with scales [experts][intermediate/128]
+ *      [hidden/128], wd [experts][hidden][intermediate]; the shared expert
+ *      (shared_intermediate > 0) one MLP of the same layout, its pointers NULL
+ *      otherwise. out [tokens][hidden] fp32 or fp16, 16-byte aligned. Sizes multiples
+ *      of 128, experts <= 1024, top_k <= 32. scratch: mpp41_moe_fp8_scratch_bytes
+ *      (0 for a descriptor that is refused), 256-byte aligned, its own for each call
+ *      in flight. ---- */
+typedef struct {
+    uint32_t tokens, hidden, intermediate;
+    uint32_t experts, top_k;
+    uint32_t shared_intermediate;
+    int32_t fmt;
+    int32_t out_f16;
+} mpp41_moe_fp8_desc;
+size_t mpp41_moe_fp8_scratch_bytes(const mpp41_moe_fp8_desc *desc);
+mpp41_status mpp41_moe_fp8(mpp41_ctx *ctx, const mpp41_moe_fp8_desc *desc, const void *x, const int32_t *ids,
+                           const float *weights, const void *wg, const float *sg, const void *wu, const float *su,
+                           const void *wd, const float *sd, const void *shared_wg, const float *shared_sg,
+                           const void *shared_wu, const float *shared_su, const void *shared_wd,
+                           const float *shared_sd, void *out, void *scratch);
+
 /* ---- tensor parallelism (no counterpart in the
  *      single-GPU reference). Rank r of P holds rows [i0, i1) of the gate and
  *      up weights (and their scale rows) and the same columns of the down

@@ -1,0 +1,153 @@
+// Host side of the FP8 block-scaled products: shape checks, tensor maps, the
+// choice of kernel and the launch.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstring>
+
+#include "mpp41_fp8_gemm.cuh"
+#include "mpp41_internal.h"
+
+namespace mpp41 {
+namespace fp8 {
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+int sm_count(int dev)
+{
+    static std::atomic<int> n[kMaxDevices];
+    int v = n[dev].load(std::memory_order_relaxed);
+    if (!v) {
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) v = 148;
+        n[dev].store(v, std::memory_order_relaxed);
+    }
+    return v;
+}
+
+template <int BN, int AR, int E, bool SPLIT> cudaError_t prepare(int dev)
+{
+    static std::atomic<uint64_t> done;
+    if (done.load(std::memory_order_acquire) >> dev & 1u) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<BN, AR, E, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(Cfg<BN, AR>::kSmem + 4 * (3 * kFp8MaxGroups + 1)));
+    if (e == cudaSuccess) done.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+}
+
+// Clusters of `parts` CTAs of the split kernel that are resident at once.
+template <int BN, int AR> int resident_clusters(int dev, int parts)
+{
+    static std::atomic<int> n[kMaxDevices][9];
+    int v = n[dev][parts].load(std::memory_order_relaxed);
+    if (!v) {
+        if (prepare<BN, AR, EPI_STORE, true>(dev) != cudaSuccess) return 0;
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute at{};
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = (unsigned)parts;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+        cfg.gridDim = dim3((unsigned)parts);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = Cfg<BN, AR>::kSmem + 4 * 4;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&v, fp8_gemm_kernel<BN, AR, EPI_STORE, true>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            v = 0;
+        }
+        v = v < 1 ? -1 : v;
+        n[dev][parts].store(v, std::memory_order_relaxed);
+    }
+    return v < 0 ? 0 : v;
+}
+
+template <int BN, int AR, int E, bool SPLIT>
+cudaError_t launch(const Params &p, int dev, uint32_t grid, uint32_t parts, cudaStream_t st)
+{
+    cudaError_t e = prepare<BN, AR, E, SPLIT>(dev);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = parts;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<BN, AR>::kSmem + 4 * (3 * p.groups + 1);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, AR, E, SPLIT>, p);
+}
+
+}  // namespace
+}  // namespace fp8
+
+int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
+{
+    using namespace fp8;
+    const bool swiglu = L.b1 != nullptr;
+    if (!L.M || !L.N || !L.groups) return 0;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev >= kMaxDevices) { *why = "device"; return 2; }
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.sa = L.sa; p.sb0 = L.sb0; p.sb1 = L.sb1;
+    p.offsets = L.offsets;
+    p.out = L.out; p.out_scales = L.out_scales;
+    p.M = L.M; p.N = L.N; p.K = L.K;
+    p.kb = (L.K + kBK - 1) / kBK;
+    p.nb = (L.N + 127) / 128;
+    p.groups = L.groups;
+    p.out_f16 = L.out_f16;
+    p.out_fmt = L.out_fmt;
+    const size_t row = (size_t)L.N * (swiglu ? 1 : L.out_f16 ? 2 : 4);
+    p.vec = row % 16 == 0 && (reinterpret_cast<uintptr_t>(L.out) & 15u) == 0;
+    p.err = L.err;
+    const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const uint64_t b_rows = (uint64_t)L.groups * L.N;
+    if (!make_map(&p.tm_a, L.a, u8, 1, L.K, L.M, kBK, kBoxRows, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !make_map(&p.tm_b0, L.b0, u8, 1, L.K, b_rows, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        (swiglu && !make_map(&p.tm_b1, L.b1, u8, 1, L.K, b_rows, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B))) {
+        *why = "tensor maps";
+        return 2;
+    }
+    const uint32_t af = L.a_fmt == 1 ? 0u : 1u, bf = L.b_fmt == 1 ? 0u : 1u;   // FMT_E4M3 = 1, FMT_E5M2 = 2
+    const uint64_t sms = (uint64_t)sm_count(dev);
+    // row tiles at most: a group's last tile may be partial
+    const uint64_t mt = L.offsets ? L.M / kBM + (L.groups < L.M ? L.groups : L.M) : (L.M + kBM - 1) / kBM;
+    if (!swiglu && !L.offsets && mt * ((L.N + 255) / 256) < sms) {
+        // Too few 128 x 256 tiles for the SMs: 128 x 128 tiles, K split over a
+        // cluster as far as its CTAs all run at once and keep four blocks each.
+        const uint64_t tiles = mt * ((L.N + 127) / 128);
+        uint32_t parts = 1;
+        for (uint32_t s = 2; s <= 8; s *= 2) {
+            const int fit = L.M <= 32 ? resident_clusters<128, 32>(dev, (int)s) : resident_clusters<128, 128>(dev, (int)s);
+            if (tiles <= (uint64_t)fit && p.kb / s >= 4) parts = s;
+        }
+        if (tiles <= sms) {
+            p.n_tiles = (L.N + 127) / 128;
+            p.idesc = idesc_f8(128, 128, af, bf);
+            const uint32_t grid = (uint32_t)(tiles * parts);
+            e = L.M <= 32 ? launch<128, 32, EPI_STORE, true>(p, dev, grid, parts, st)
+                          : launch<128, 128, EPI_STORE, true>(p, dev, grid, parts, st);
+            if (e != cudaSuccess) { cudaGetLastError(); *why = cudaGetErrorString(e); return 2; }
+            return 0;
+        }
+    }
+    const uint32_t cols = swiglu ? 128 : 256;
+    p.n_tiles = (L.N + cols - 1) / cols;
+    p.idesc = idesc_f8(128, 256, af, bf);
+    const uint64_t bound = mt * p.n_tiles;
+    if (bound >> 32) { *why = "too many tiles"; return 1; }
+    const uint32_t grid = (uint32_t)(bound < sms ? bound : sms);
+    e = swiglu ? launch<256, 128, EPI_SWIGLU, false>(p, dev, grid, 1, st) : launch<256, 128, EPI_STORE, false>(p, dev, grid, 1, st);
+    if (e != cudaSuccess) { cudaGetLastError(); *why = cudaGetErrorString(e); return 2; }
+    return 0;
+}
+
+}  // namespace mpp41

@@ -109,6 +109,54 @@ struct MxLaunch {
 };
 int launch_mxf4_gemm(const MxLaunch &L, cudaStream_t st, const char **why);
 
+// FP8 products with fp32 scales per block of 128 (mpp41_fp8_gemm.cuh): A [M][K]
+// with scales [M][K/128], B [groups * N][K] with scales [groups][N/128][K/128];
+// rows [offsets[g], offsets[g+1]) meet B[g] (offsets null: one group). With b1
+// (the up weights beside the gate weights b0) the result is silu(gate) * up as
+// 8-bit values [M][N] of out_fmt with scales [M][N/128] (N % 128 == 0).
+// K % 16 == 0, A and B 16-byte aligned, groups <= kFp8MaxGroups.
+constexpr uint32_t kFp8MaxGroups = 1024;
+struct Fp8Launch {
+    const void *a, *b0, *b1;
+    const float *sa, *sb0, *sb1;
+    const int32_t *offsets;
+    void *out;
+    float *out_scales;
+    uint32_t M, N, K, groups;
+    int a_fmt, b_fmt, out_fmt;   // FMT_E4M3 (1) or FMT_E5M2 (2)
+    int out_f16;
+    uint32_t *err;
+};
+int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why);
+// FP8 quantizers (mpp41_fp8_quant.cu): fp16 [T][H] with a scale per 1 x 128, fp32
+// [N][K] with a scale per 128 x 128 (ceil(N/128) * ceil(K/128) < 2^31).
+cudaError_t launch_quantize_act_fp8(int fmt, const void *x, uint32_t T, uint32_t H, uint8_t *q, float *scales,
+                                    cudaStream_t st);
+cudaError_t launch_quantize_weights_fp8(int fmt, const float *w, uint32_t N, uint32_t K, uint8_t *q, float *scales,
+                                        cudaStream_t st);
+
+// Pieces of the FP8 expert layer (mpp41_moe_fp8.cu): n = T * k assignments; H % 128 == 0,
+// x 32-byte aligned; xq / xs (the unscattered rows) may be null.
+cudaError_t launch_fp8_plan(const int32_t *ids, uint32_t n, uint32_t E, int32_t *offsets, int32_t *inv, uint32_t *err,
+                            cudaStream_t st);
+cudaError_t launch_fp8_scatter(int fmt, const void *x, uint32_t T, uint32_t H, const int32_t *inv, uint32_t k, uint8_t *pq,
+                               float *ps, uint8_t *xq, float *xs, cudaStream_t st);
+cudaError_t launch_fp8_combine(const float *y, const int32_t *inv, const float *w, uint32_t T, uint32_t k, uint32_t H,
+                               const float *shared_y, void *out, int out_f16, cudaStream_t st);
+
+// Expert routing with scores, balance bias and groups (mpp41_moe_gate.cu): E <= 512,
+// k <= 32, groups <= 32 dividing E.
+struct GateLaunch {
+    const void *logits;
+    const float *bias;
+    int32_t *ids;
+    float *weights;
+    uint32_t T, E, k, groups, top_groups, group_top;
+    int sigmoid, renorm, f16;
+    float scale;
+};
+cudaError_t launch_moe_gate(const GateLaunch &L, cudaStream_t st);
+
 // Mixture-of-experts pieces (mpp41_moe.cu).
 cudaError_t launch_moe_route(const float *logits, uint32_t T, uint32_t E, uint32_t k, int32_t *ids, float *weights,
                              cudaStream_t st);

@@ -1,0 +1,165 @@
+// The pieces of the FP8 expert layer around its two grouped products
+// (mpp41_fp8_gemm.cuh), for T tokens, k assignments a token, E experts:
+//   plan:     ids [T][k] -> offsets[E+1] (rows of each expert) and inv[T*k]
+//             (assignment -> row, -1 where the id names no expert). Rows are grouped
+//             by expert and keep assignment order inside one: deterministic.
+//   scatter:  x is quantized once (1 x 128 scales) and each block written to the
+//             rows of its token's assignments; no gather pass reads it again.
+//   experts:  grouped gate/up product with the SwiGLU + quantization epilogue, then
+//             the grouped down product -> y [rows][H] fp32.
+//   combine:  out[t] = shared(t) + sum_j weights[t][j] * y[inv[t*k+j]], in slot order.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "mpp41_device.cuh"
+#include "mpp41_fp8.cuh"
+#include "mpp41_internal.h"
+
+namespace mpp41 {
+namespace fp8 {
+
+constexpr int kPlanThreads = 512;
+
+// One CTA an expert, each reading all ids twice (they sit in L2): rows before this
+// expert's = ids below it, then a stable compaction. Threads own contiguous runs
+// of assignments, so one block scan orders them. No launch or wait joins the CTAs.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__restrict__ ids, uint32_t n, uint32_t E,
+                                                            int32_t *__restrict__ offsets, int32_t *__restrict__ inv,
+                                                            uint32_t *err)
+{
+    __shared__ uint32_t sh_lt[kPlanThreads / 32], sh_eq[kPlanThreads / 32];
+    const int32_t e = (int32_t)blockIdx.x;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t per = (n + kPlanThreads - 1) / kPlanThreads;
+    const uint32_t a0 = min(threadIdx.x * per, n), a1 = min(a0 + per, n);
+    uint32_t lt = 0, eq = 0;
+    bool bad = false;
+    for (uint32_t a = a0; a < a1; ++a) {
+        const int32_t id = ids[a];
+        lt += id >= 0 && id < e;
+        eq += id == e;
+        if (e == 0 && (id < 0 || id >= (int32_t)E)) {
+            inv[a] = -1;
+            bad |= id >= (int32_t)E;
+        }
+    }
+    if (bad) report_error(err, kErrBounds, 0xF91);
+    uint32_t inc = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= (uint32_t)o) inc += v;
+    }
+    lt = __reduce_add_sync(0xffffffffu, lt);
+    if (lane == 31) {
+        sh_lt[warp] = lt;
+        sh_eq[warp] = inc;
+    }
+    __syncthreads();
+    uint32_t base = 0, all = 0, before = 0;
+    for (uint32_t w = 0; w < kPlanThreads / 32; ++w) {
+        base += sh_lt[w];
+        all += sh_eq[w];
+        before += w < warp ? sh_eq[w] : 0u;
+    }
+    if (threadIdx.x == 0) {
+        offsets[e] = (int32_t)base;
+        if (e == (int32_t)E - 1) offsets[E] = (int32_t)(base + all);
+    }
+    uint32_t row = base + before + inc - eq;
+    if (eq)
+        for (uint32_t a = a0; a < a1; ++a)
+            if (ids[a] == e) inv[a] = (int32_t)row++;
+}
+
+// As the activation quantizer (8 lanes a block of 128, 16 values a lane), each block
+// written to the rows inv[t*k + j] >= 0 and, where xq is given, to row t of xq.
+template <int FMT>
+__global__ void __launch_bounds__(256) quant_scatter_kernel(const uint8_t *__restrict__ x, uint32_t kb, uint64_t blocks,
+                                                            const int32_t *__restrict__ inv, uint32_t k,
+                                                            uint8_t *__restrict__ pq, float *__restrict__ ps,
+                                                            uint8_t *__restrict__ xq, float *__restrict__ xs)
+{
+    const uint32_t sub = threadIdx.x & 7;
+    const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 8);
+    for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 8) + threadIdx.x / 8; __any_sync(0xffffffffu, i < blocks); i += step) {
+        const bool have = i < blocks;
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = 0u;
+        if (have) load_act16(x + (i * 128 + sub * 16) * 2, w);
+        float scale;
+        const uint4 o = quant_act16<FMT>(w, scale);
+        if (!have) continue;
+        const uint64_t t = i / kb;
+        const uint32_t b = (uint32_t)(i - t * kb);
+        if (xq) {
+            *reinterpret_cast<uint4 *>(xq + i * 128 + sub * 16) = o;
+            if (sub == 0) xs[i] = scale;
+        }
+        for (uint32_t j = 0; j < k; ++j) {
+            const int32_t r = inv[t * k + j];
+            if (r < 0) continue;
+            const uint64_t at = (uint64_t)r * kb + b;
+            *reinterpret_cast<uint4 *>(pq + at * 128 + sub * 16) = o;
+            if (sub == 0) ps[at] = scale;
+        }
+    }
+}
+
+// One CTA per (token, 1024 columns); slots summed in order, fp32.
+__global__ void __launch_bounds__(256) combine_fp8_kernel(const float *__restrict__ y, const int32_t *__restrict__ inv,
+                                                          const float *__restrict__ w, uint32_t k, uint32_t H,
+                                                          const float *__restrict__ shared_y, void *__restrict__ out, int out_f16)
+{
+    const uint32_t t = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
+    if (c >= H / 4) return;
+    float4 acc = shared_y ? __ldcs(reinterpret_cast<const float4 *>(shared_y + (size_t)t * H) + c) : make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (uint32_t j = 0; j < k; ++j) {
+        const int32_t r = inv[(size_t)t * k + j];
+        if (r < 0) continue;
+        const float wt = w[(size_t)t * k + j];
+        const float4 v = __ldcs(reinterpret_cast<const float4 *>(y + (size_t)r * H) + c);
+        acc.x = fmaf(wt, v.x, acc.x);
+        acc.y = fmaf(wt, v.y, acc.y);
+        acc.z = fmaf(wt, v.z, acc.z);
+        acc.w = fmaf(wt, v.w, acc.w);
+    }
+    if (out_f16)
+        reinterpret_cast<uint2 *>(static_cast<__half *>(out) + (size_t)t * H)[c] = make_uint2(half2_bits(acc.x, acc.y), half2_bits(acc.z, acc.w));
+    else
+        reinterpret_cast<float4 *>(static_cast<float *>(out) + (size_t)t * H)[c] = acc;
+}
+
+}  // namespace fp8
+
+cudaError_t launch_fp8_plan(const int32_t *ids, uint32_t n, uint32_t E, int32_t *offsets, int32_t *inv, uint32_t *err,
+                            cudaStream_t st)
+{
+    fp8::plan_kernel<<<E, fp8::kPlanThreads, 0, st>>>(ids, n, E, offsets, inv, err);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_fp8_scatter(int fmt, const void *x, uint32_t T, uint32_t H, const int32_t *inv, uint32_t k, uint8_t *pq,
+                               float *ps, uint8_t *xq, float *xs, cudaStream_t st)
+{
+    const uint64_t blocks = (uint64_t)T * (H / 128), need = (blocks + 31) / 32;
+    const unsigned grid = (unsigned)(need < 148 * 16 ? need : 148 * 16);
+    const uint8_t *xb = static_cast<const uint8_t *>(x);
+    if (fmt == 1) fp8::quant_scatter_kernel<1><<<grid, 256, 0, st>>>(xb, H / 128, blocks, inv, k, pq, ps, xq, xs);
+    else fp8::quant_scatter_kernel<2><<<grid, 256, 0, st>>>(xb, H / 128, blocks, inv, k, pq, ps, xq, xs);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_fp8_combine(const float *y, const int32_t *inv, const float *w, uint32_t T, uint32_t k, uint32_t H,
+                               const float *shared_y, void *out, int out_f16, cudaStream_t st)
+{
+    const dim3 grid(T, (H / 4 + 255) / 256);
+    fp8::combine_fp8_kernel<<<grid, 256, 0, st>>>(y, inv, w, k, H, shared_y, out, out_f16);
+    return cudaGetLastError();
+}
+
+}  // namespace mpp41

@@ -32,6 +32,7 @@ F32, F16, S32, S8 = range(4)
 MLP_UNFUSED = 0x1
 MLP_ROW_SCALES = 0x2
 FMT_E2M1, FMT_E4M3, FMT_E5M2 = 0, 1, 2
+GATE_SOFTMAX, GATE_SIGMOID = 0, 1
 
 
 class MPP41Error(RuntimeError):
@@ -59,6 +60,18 @@ class MoEDesc(C.Structure):
     _fields_ = [("tokens", C.c_uint32), ("hidden", C.c_uint32), ("intermediate", C.c_uint32),
                 ("experts", C.c_uint32), ("top_k", C.c_uint32), ("shared_intermediate", C.c_uint32),
                 ("out_f16", C.c_int32)]
+
+
+class GateDesc(C.Structure):
+    _fields_ = [("tokens", C.c_uint32), ("experts", C.c_uint32), ("top_k", C.c_uint32), ("score", C.c_int32),
+                ("groups", C.c_uint32), ("top_groups", C.c_uint32), ("group_top", C.c_uint32),
+                ("renormalize", C.c_int32), ("scale", C.c_float), ("logits_f16", C.c_int32)]
+
+
+class MoEFP8Desc(C.Structure):
+    _fields_ = [("tokens", C.c_uint32), ("hidden", C.c_uint32), ("intermediate", C.c_uint32),
+                ("experts", C.c_uint32), ("top_k", C.c_uint32), ("shared_intermediate", C.c_uint32),
+                ("fmt", C.c_int32), ("out_f16", C.c_int32)]
 
 
 MOE_PARTS = ("xq", "xs", "ids", "weights", "counts", "offsets", "n_tiles", "tiles", "perm", "inv", "pq", "ps",
@@ -134,6 +147,13 @@ def lib() -> C.CDLL:
         "mpp41_mlp_w8a8": ([vp, C.c_int, u32, u32, u32] + [vp] * 9, st),
         "mpp41_moe_route": ([vp, vp, u32, u32, u32, vp, vp], st),
         "mpp41_moe_w4a4": ([vp, C.POINTER(MoEDesc)] + [vp] * 16, st),
+        "mpp41_moe_gate": ([vp, C.POINTER(GateDesc)] + [vp] * 4, st),
+        "mpp41_quantize_act_fp8": ([vp, C.c_int, vp, u32, u32, vp, vp], st),
+        "mpp41_quantize_weights_fp8": ([vp, C.c_int, vp, u32, u32, vp, vp], st),
+        "mpp41_matmul_fp8": ([vp, C.c_int, vp, vp, C.c_int, vp, vp, vp, u32, u32, u32, C.c_int], st),
+        "mpp41_matmul_fp8_grouped": ([vp, C.c_int, vp, vp, C.c_int, vp, vp, vp, u32, vp, u32, u32, u32, C.c_int], st),
+        "mpp41_moe_fp8_scratch_bytes": ([C.POINTER(MoEFP8Desc)], sz),
+        "mpp41_moe_fp8": ([vp, C.POINTER(MoEFP8Desc)] + [vp] * 17, st),
         "mpp41_moe_ep_scratch_layout": ([C.POINTER(MoEDesc), C.c_int, u32, vp], sz),
         "mpp41_moe_ep": ([vp, C.POINTER(MoEDesc), u32] + [vp] * 16, st),
         "mpp41_mlp_nvfp4": ([vp, u32, u32, u32] + [vp] * 11 + [C.c_int, vp], st),
@@ -222,6 +242,26 @@ def moe_scratch_layout(desc: MoEDesc):
 
 def moe_ep_scratch_bytes(desc: MoEDesc, nranks: int, capacity: int) -> int:
     return lib().mpp41_moe_ep_scratch_layout(C.byref(desc), nranks, capacity, None)
+
+
+def gate_desc(tokens, experts, top_k, score=GATE_SOFTMAX, groups=1, top_groups=1, group_top=1, renormalize=True,
+              scale=1.0, logits_f16=False) -> GateDesc:
+    return GateDesc(tokens, experts, top_k, score, groups, top_groups, group_top, int(renormalize), scale,
+                    int(logits_f16))
+
+
+def moe_fp8_desc(tokens, hidden, intermediate, experts, top_k, shared_intermediate=0, fmt=FMT_E4M3,
+                 out_f16=False) -> MoEFP8Desc:
+    return MoEFP8Desc(tokens, hidden, intermediate, experts, top_k, shared_intermediate, fmt, int(out_f16))
+
+
+def moe_fp8_scratch_bytes(desc: MoEFP8Desc) -> int:
+    """Scratch of Context.moe_fp8; raises where the descriptor is refused."""
+    n = lib().mpp41_moe_fp8_scratch_bytes(C.byref(desc))
+    if n == 0:
+        msg = lib().mpp41_last_error()
+        raise MPP41Error(ERR_UNSUPPORTED_SHAPE, msg.decode() if msg else "")
+    return n
 
 
 def w8a8_scratch_bytes(tokens: int, hidden: int, intermediate: int) -> int:
@@ -488,6 +528,36 @@ class Context:
         sh = [_ptr(v) for v in shared] if shared is not None else [None] * 6
         _check(lib().mpp41_moe_ep(self.h, C.byref(desc), capacity, _ptr(x), _ptr(logits), _ptr(wg), _ptr(sg),
                                   _ptr(wu), _ptr(su), _ptr(wd), _ptr(sd), *sh, _ptr(out), _ptr(scratch)))
+
+    def moe_gate(self, desc: GateDesc, logits, bias, ids, weights):
+        """Expert ids and weights of each token (mpp41_moe_gate); bias may be None."""
+        _check(lib().mpp41_moe_gate(self.h, C.byref(desc), _ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights)))
+
+    def quantize_act_fp8(self, fmt: int, x, tokens: int, hidden: int, q, scales):
+        """fp16 activations -> FP8 with a scale per 1 x 128 (mpp41_quantize_act_fp8)."""
+        _check(lib().mpp41_quantize_act_fp8(self.h, fmt, _ptr(x), tokens, hidden, _ptr(q), _ptr(scales)))
+
+    def quantize_weights_fp8(self, fmt: int, w, rows: int, depth: int, q, scales):
+        """fp32 weights -> FP8 with a scale per 128 x 128 (mpp41_quantize_weights_fp8)."""
+        _check(lib().mpp41_quantize_weights_fp8(self.h, fmt, _ptr(w), rows, depth, _ptr(q), _ptr(scales)))
+
+    def matmul_fp8(self, a_fmt: int, a, sa, b_fmt: int, b, sb, c, M: int, N: int, K: int, c_f16: bool = False):
+        """C[M][N] = A[M][K] B[N][K]^T, FP8 with fp32 scales per block of 128 (mpp41_matmul_fp8)."""
+        _check(lib().mpp41_matmul_fp8(self.h, a_fmt, _ptr(a), _ptr(sa), b_fmt, _ptr(b), _ptr(sb), _ptr(c), M, N, K,
+                                      int(c_f16)))
+
+    def matmul_fp8_grouped(self, a_fmt: int, a, sa, b_fmt: int, b, sb, offsets, groups: int, c, M: int, N: int, K: int,
+                           c_f16: bool = False):
+        """The same with B[g] for rows [offsets[g], offsets[g+1]) (mpp41_matmul_fp8_grouped); offsets int32 on the device."""
+        _check(lib().mpp41_matmul_fp8_grouped(self.h, a_fmt, _ptr(a), _ptr(sa), b_fmt, _ptr(b), _ptr(sb), _ptr(offsets),
+                                              groups, _ptr(c), M, N, K, int(c_f16)))
+
+    def moe_fp8(self, desc: MoEFP8Desc, x, ids, weights, wg, sg, wu, su, wd, sd, out, scratch, shared=None):
+        """One FP8 expert layer (mpp41_moe_fp8); shared = (wg, sg, wu, su, wd, sd) or None, scratch of
+        moe_fp8_scratch_bytes()."""
+        sh = [_ptr(v) for v in shared] if shared is not None else [None] * 6
+        _check(lib().mpp41_moe_fp8(self.h, C.byref(desc), _ptr(x), _ptr(ids), _ptr(weights), _ptr(wg), _ptr(sg), _ptr(wu),
+                                   _ptr(su), _ptr(wd), _ptr(sd), *sh, _ptr(out), _ptr(scratch)))
 
     def quantize_weights_int(self, w, rows: int, depth: int, bits: int, packed, scales):
         """fp32 weights -> per-row symmetric INT8/INT4/INT2 + fp32 row scales (mpp41_quantize_weights_int)."""
