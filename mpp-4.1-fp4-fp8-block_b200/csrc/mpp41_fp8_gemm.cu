@@ -27,12 +27,12 @@ int sm_count(int dev)
     return v;
 }
 
-template <int BN, int AR, int E, bool SPLIT> cudaError_t prepare(int dev)
+template <int BN, int AR, int E, int MODE> cudaError_t prepare(int dev)
 {
     static std::atomic<uint64_t> done;
     if (done.load(std::memory_order_acquire) >> dev & 1u) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<BN, AR, E, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)(Cfg<BN, AR>::kSmem + 4 * (3 * kFp8MaxGroups + 1)));
+    const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<BN, AR, E, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(Cfg<BN, AR, MODE>::kSmem + 4 * (3 * kFp8MaxGroups + 1)));
     if (e == cudaSuccess) done.fetch_or(1ull << dev, std::memory_order_release);
     return e;
 }
@@ -43,7 +43,7 @@ template <int BN, int AR> int resident_clusters(int dev, int parts)
     static std::atomic<int> n[kMaxDevices][9];
     int v = n[dev][parts].load(std::memory_order_relaxed);
     if (!v) {
-        if (prepare<BN, AR, EPI_STORE, true>(dev) != cudaSuccess) return 0;
+        if (prepare<BN, AR, EPI_STORE, SPLIT>(dev) != cudaSuccess) return 0;
         cudaLaunchConfig_t cfg{};
         cudaLaunchAttribute at{};
         at.id = cudaLaunchAttributeClusterDimension;
@@ -51,10 +51,10 @@ template <int BN, int AR> int resident_clusters(int dev, int parts)
         at.val.clusterDim.y = at.val.clusterDim.z = 1;
         cfg.gridDim = dim3((unsigned)parts);
         cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = Cfg<BN, AR>::kSmem + 4 * 4;
+        cfg.dynamicSmemBytes = Cfg<BN, AR, SPLIT>::kSmem + 4 * 4;
         cfg.attrs = &at;
         cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&v, fp8_gemm_kernel<BN, AR, EPI_STORE, true>, &cfg) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&v, fp8_gemm_kernel<BN, AR, EPI_STORE, SPLIT>, &cfg) != cudaSuccess) {
             cudaGetLastError();
             v = 0;
         }
@@ -64,10 +64,10 @@ template <int BN, int AR> int resident_clusters(int dev, int parts)
     return v < 0 ? 0 : v;
 }
 
-template <int BN, int AR, int E, bool SPLIT>
+template <int BN, int AR, int E, int MODE>
 cudaError_t launch(const Params &p, int dev, uint32_t grid, uint32_t parts, cudaStream_t st)
 {
-    cudaError_t e = prepare<BN, AR, E, SPLIT>(dev);
+    cudaError_t e = prepare<BN, AR, E, MODE>(dev);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
@@ -76,11 +76,11 @@ cudaError_t launch(const Params &p, int dev, uint32_t grid, uint32_t parts, cuda
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Cfg<BN, AR>::kSmem + 4 * (3 * p.groups + 1);
+    cfg.dynamicSmemBytes = Cfg<BN, AR, MODE>::kSmem + 4 * (3 * p.groups + 1);
     cfg.stream = st;
     cfg.attrs = &at;
-    cfg.numAttrs = SPLIT ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, AR, E, SPLIT>, p);
+    cfg.numAttrs = MODE == SINGLE ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, AR, E, MODE>, p);
 }
 
 }  // namespace
@@ -108,6 +108,13 @@ int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
     const size_t row = (size_t)L.N * (swiglu ? 1 : L.out_f16 ? 2 : 4);
     p.vec = row % 16 == 0 && (reinterpret_cast<uintptr_t>(L.out) & 15u) == 0;
     p.err = L.err;
+    // Row tiles at most (a group's last may be partial), of 128 rows and of a pair's 256.
+    // Pairs where groups fill more than one row tile on average: the half of a pair that
+    // has no rows would only move weights.
+    const uint64_t mt = L.offsets ? L.M / kBM + (L.groups < L.M ? L.groups : L.M) : (L.M + kBM - 1) / kBM;
+    const uint64_t sms = (uint64_t)sm_count(dev);
+    const bool few = !swiglu && !L.offsets && mt * ((L.N + 255) / 256) < sms && mt * ((L.N + 127) / 128) <= sms;
+    const bool pair = !few && L.M / L.groups > 128;
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const uint64_t b_rows = (uint64_t)L.groups * L.N;
     if (!make_map(&p.tm_a, L.a, u8, 1, L.K, L.M, kBK, kBoxRows, CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -117,10 +124,8 @@ int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
         return 2;
     }
     const uint32_t af = L.a_fmt == 1 ? 0u : 1u, bf = L.b_fmt == 1 ? 0u : 1u;   // FMT_E4M3 = 1, FMT_E5M2 = 2
-    const uint64_t sms = (uint64_t)sm_count(dev);
-    // row tiles at most: a group's last tile may be partial
-    const uint64_t mt = L.offsets ? L.M / kBM + (L.groups < L.M ? L.groups : L.M) : (L.M + kBM - 1) / kBM;
-    if (!swiglu && !L.offsets && mt * ((L.N + 255) / 256) < sms) {
+    p.idesc = idesc_f8(pair ? 256 : 128, few ? 128 : 256, af, bf);
+    if (few) {
         // Too few 128 x 256 tiles for the SMs: 128 x 128 tiles, K split over a
         // cluster as far as its CTAs all run at once and keep four blocks each.
         const uint64_t tiles = mt * ((L.N + 127) / 128);
@@ -129,23 +134,23 @@ int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
             const int fit = L.M <= 32 ? resident_clusters<128, 32>(dev, (int)s) : resident_clusters<128, 128>(dev, (int)s);
             if (tiles <= (uint64_t)fit && p.kb / s >= 4) parts = s;
         }
-        if (tiles <= sms) {
-            p.n_tiles = (L.N + 127) / 128;
-            p.idesc = idesc_f8(128, 128, af, bf);
-            const uint32_t grid = (uint32_t)(tiles * parts);
-            e = L.M <= 32 ? launch<128, 32, EPI_STORE, true>(p, dev, grid, parts, st)
-                          : launch<128, 128, EPI_STORE, true>(p, dev, grid, parts, st);
-            if (e != cudaSuccess) { cudaGetLastError(); *why = cudaGetErrorString(e); return 2; }
-            return 0;
-        }
+        p.n_tiles = (L.N + 127) / 128;
+        const uint32_t grid = (uint32_t)(tiles * parts);
+        e = L.M <= 32 ? launch<128, 32, EPI_STORE, SPLIT>(p, dev, grid, parts, st)
+                      : launch<128, 128, EPI_STORE, SPLIT>(p, dev, grid, parts, st);
+        if (e != cudaSuccess) { cudaGetLastError(); *why = cudaGetErrorString(e); return 2; }
+        return 0;
     }
     const uint32_t cols = swiglu ? 128 : 256;
     p.n_tiles = (L.N + cols - 1) / cols;
-    p.idesc = idesc_f8(128, 256, af, bf);
-    const uint64_t bound = mt * p.n_tiles;
-    if (bound >> 32) { *why = "too many tiles"; return 1; }
-    const uint32_t grid = (uint32_t)(bound < sms ? bound : sms);
-    e = swiglu ? launch<256, 128, EPI_SWIGLU, false>(p, dev, grid, 1, st) : launch<256, 128, EPI_STORE, false>(p, dev, grid, 1, st);
+    const uint64_t bound = pair ? (L.offsets ? L.M / 256 + L.groups : (L.M + 255) / 256) * (uint64_t)p.n_tiles : mt * p.n_tiles;
+    if (bound >> 31) { *why = "too many tiles"; return 1; }
+    const uint64_t fit = pair ? sms / 2 : sms;
+    const uint32_t grid = (uint32_t)(bound < fit ? bound : fit) * (pair ? 2 : 1);
+    if (pair)
+        e = swiglu ? launch<256, 128, EPI_SWIGLU, PAIR>(p, dev, grid, 2, st) : launch<256, 128, EPI_STORE, PAIR>(p, dev, grid, 2, st);
+    else
+        e = swiglu ? launch<256, 128, EPI_SWIGLU, SINGLE>(p, dev, grid, 1, st) : launch<256, 128, EPI_STORE, SINGLE>(p, dev, grid, 1, st);
     if (e != cudaSuccess) { cudaGetLastError(); *why = cudaGetErrorString(e); return 2; }
     return 0;
 }

@@ -17,8 +17,11 @@
 // pair instead of a shared-memory read per column. Row blocks past the tile's end
 // are neither loaded nor promoted (32-row granularity).
 //
-// Warp roles (384 threads): 0 TMA producer, 1 MMA issuer and TMEM owner, 2..3
-// idle, 4..11 promotion (warp w: TMEM lane quarter w % 4, column half (w - 4) / 4).
+// Warp roles (384 threads): 0 TMA producer, 1 MMA issuer and TMEM owner, 2..3 idle (they
+// hold registers that the promotion warps take over), 4..11 promotion (warp w: TMEM lane
+// quarter w % 4, column half (w - 4) / 4). One warp for copies and MMAs ran the
+// 4096 x 14336 x 4096 product a third slower: a block's copies take it as long to issue
+// as the block's MMAs take to run.
 #pragma once
 
 #include <cuda.h>
@@ -41,22 +44,31 @@ constexpr uint32_t kBoxBytes = kBoxRows * kBK;
 constexpr uint32_t kBTile = 128 * kBK;      // 128 rows of B
 
 enum Epi { EPI_STORE = 0, EPI_SWIGLU = 1 };
+// SINGLE: one CTA a tile, persistent. PAIR: two CTAs of a cluster share a 256-row tile:
+// tcgen05 cta_group::2 with M = 256, each CTA holding its 128 rows of A and half of B's
+// columns, so a K block brings 32 KB into each SM instead of 48 KB; persistent. SPLIT:
+// one tile a cluster, its CTAs take ranges of K blocks.
+enum Mode { SINGLE = 0, PAIR = 1, SPLIT = 2 };
 
 // AR: rows of A a stage has room for. With AR = 32 (at most 32 rows in the whole
 // launch) the MMA still reads 128 rows from the stage's start: the other 96 come
 // from the neighbouring stages and only reach accumulator lanes nobody reads.
-template <int BN, int AR> struct Cfg {
+template <int BN, int AR, int MODE> struct Cfg {
+    static constexpr uint32_t kRuns = BN / 128;                     // runs of 128 columns, each with its scale of B
+    static constexpr uint32_t kTileRows = MODE == PAIR ? 256 : 128;
     static constexpr uint32_t kAStage = AR * kBK;
-    static constexpr uint32_t kBStage = BN * kBK;
-    static constexpr int kStages = BN == 256 ? 4 : (AR == 32 ? 9 : 6);
+    static constexpr uint32_t kBStage = (MODE == PAIR ? 1 : kRuns) * kBTile;   // PAIR: run `rank` only
+    static constexpr int kStages = MODE == PAIR ? 6 : BN == 256 ? 4 : (AR == 32 ? 9 : 6);
     static constexpr uint32_t kOffB = ((kStages * kAStage + 1023) / 1024) * 1024;
-    static constexpr uint32_t kOffBar = kOffB + kStages * kBStage;
-    static constexpr uint32_t kOffAmax = kOffBar + 256;             // SwiGLU: [2 tiles][2 halves][128] floats
-    static constexpr uint32_t kOffGroups = kOffAmax + 2048;         // 3 words per group + 1
-    static constexpr uint32_t kSmem = 1024 + kOffGroups;            // + 4 * (3 * groups + 1)
+    static constexpr uint32_t kOffOut = kOffB + kStages * kBStage;  // 8 warps x 2 KB, epilogue transposition
+    static constexpr uint32_t kOffAmax = kOffOut + 8 * 2048;        // SwiGLU: [2 halves][128] floats
+    static constexpr uint32_t kOffBar = kOffAmax + 1024;
+    static constexpr uint32_t kOffGroups = kOffBar + 256;           // 3 words per group + 1
+    static constexpr uint32_t kSmem = kOffGroups;                   // + 4 * (3 * groups + 1)
     static constexpr uint32_t kTmemCols = 2 * BN;
     static_assert(AR * kBK * (kStages - 1) + 128 * kBK <= kOffB + kStages * kBStage, "MMA reads stay inside the ring");
-    static_assert(kSmem <= 227 * 1024 - 4 * (3 * 1024 + 1), "shared memory");
+    static_assert(kSmem + 4 * (3 * kFp8MaxGroups + 1) <= 227 * 1024, "shared memory");
+    static_assert(8 * (2 * kStages + 5) + 8 <= 256, "barriers");
 };
 
 struct Params {
@@ -75,6 +87,40 @@ struct Params {
     uint32_t *err;
 };
 
+// Bounded wait for the handshakes between the MMA issuer and the promotion warps. The
+// bound is a number of tries, each suspended for at most kTryNs by the hardware: about
+// kWaitLimitNs in all, and no timer to keep in the promotion warps' last registers.
+constexpr uint32_t kTryNs = 4096, kTries = (uint32_t)(kWaitLimitNs / kTryNs);
+
+__device__ __forceinline__ bool try_wait_ns(uint32_t addr, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(addr), "r"(parity), "n"(kTryNs) : "memory");
+    return ok != 0;
+}
+
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err, uint32_t site)
+{
+    const uint32_t addr = smem_u32(bar);
+    for (uint32_t it = 0; it < kTries; ++it) {
+        if (try_wait_ns(addr, parity)) return true;
+        if (*abort) return false;
+    }
+    report_error(err, kErrTimeout, site);
+    *abort = 1;
+    return false;
+}
+
+// By all lanes of a converged warp, with one outcome.
+__device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err, uint32_t site)
+{
+    return __all_sync(0xffffffffu, wait(bar, parity, abort, err, site));
+}
+
 // Instruction descriptor, kind::f8f6f4, fp32 D, both operands K-major; formats 0 = E4M3, 1 = E5M2.
 __host__ __device__ constexpr uint32_t idesc_f8(int M, int N, uint32_t af, uint32_t bf)
 {
@@ -91,6 +137,69 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t
         : "memory");
 }
 
+// ---- CTA pairs: see Mode. Barriers that the MMA issuer (even CTA) waits on live in the
+// even CTA; the odd one arrives on them through shared::cluster addresses. What they
+// order is copies and tensor-memory accesses (tcgen05 fences), no generic memory, so
+// the arrivals and waits keep the CTA's scope: with cluster scope each one flushed
+// stores or dropped L1 lines, and the 4096 x 14336 x 4096 product ran at 572 us.
+__device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t cta_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// Address of the same shared-memory object in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(const void *local, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ void arrive_cl(uint32_t caddr)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
+}
+
+__device__ __forceinline__ void arrive_expect_tx_cl(uint32_t caddr, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(caddr), "r"(bytes) : "memory");
+}
+
+// Tiled load into this CTA's shared memory, counted on an mbarrier of either CTA of the pair (no multicast).
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const void *tmap, int32_t c0, int32_t c1, uint32_t bar_caddr)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_u32(dst)), "l"(tmap), "r"(c0), "r"(c1), "r"(bar_caddr)
+        : "memory");
+}
+
+// Arrive on this barrier of both CTAs once all MMAs this thread issued before complete.
+__device__ __forceinline__ void commit_pair(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_u32(bar)), "h"((uint16_t)3)
+                 : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Completion of this thread's tcgen05.ld, tied to the registers it fills so that no use moves above it.
 __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32])
 {
@@ -103,29 +212,12 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32])
                  : "memory");
 }
 
-// acc[i] += d[2i..2i+1] * s for 16 fp32 pairs (packed fp32 FMA: two per instruction).
-__device__ __forceinline__ void promote32(uint64_t *acc, const uint32_t (&d)[32], uint64_t s2)
+// acc[i] += d[i] * s. Scalar FMAs: the packed fp32 form needs its operands moved into
+// register pairs, and ran the 4096 x 14336 x 4096 product at 400 us against 292 us.
+__device__ __forceinline__ void promote32(float *acc, const uint32_t (&d)[32], float s)
 {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        uint64_t v;
-        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(d[2 * i]), "r"(d[2 * i + 1]));
-        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i]) : "l"(v), "l"(s2));
-    }
-}
-
-__device__ __forceinline__ uint64_t pack2(float s)
-{
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(s));
-    return v;
-}
-
-__device__ __forceinline__ float2 unpack2(uint64_t v)
-{
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
+    for (int i = 0; i < 32; ++i) acc[i] = fmaf(__uint_as_float(d[i]), s, acc[i]);
 }
 
 // Barrier of the promotion warps that also ORs a flag.
@@ -154,6 +246,7 @@ struct Tile {
 
 // Tile t: groups in order; inside a group the row tile runs fastest, so that the
 // CTAs of a wave share the weight tile they stream.
+template <uint32_t ROWS>
 __device__ __forceinline__ Tile tile_at(const Params &p, const Groups &gr, uint32_t t, uint32_t cols)
 {
     uint32_t lo = 0, hi = p.groups;   // cum[lo] * n_tiles <= t < cum[hi] * n_tiles
@@ -165,7 +258,7 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const Groups &gr, uint3
     const uint32_t l = t - gr.cum[lo] * p.n_tiles;
     Tile o;
     o.g = lo;
-    o.m0 = gr.row0[lo] + (l % mt) * kBM;
+    o.m0 = gr.row0[lo] + (l % mt) * ROWS;
     o.m_end = gr.row1[lo];
     o.n0 = (l / mt) * cols;
     return o;
@@ -173,6 +266,7 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const Groups &gr, uint3
 
 // Prefix sums of the groups' row tiles (one warp). Offsets are clamped to [0, M]
 // and made ascending, so wrong ones are reported but never lead out of A or C.
+template <uint32_t ROWS>
 __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uint32_t *row0, uint32_t *row1, uint32_t lane)
 {
     const uint32_t per = (p.groups + 31) / 32;
@@ -190,7 +284,7 @@ __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uin
         }
         row0[g] = a;
         row1[g] = b;
-        sum += (b - a + kBM - 1) / kBM;
+        sum += (b - a + ROWS - 1) / ROWS;
     }
     if (bad && blockIdx.x == 0) report_error(p.err, kErrBounds, 0xF81);
     uint32_t inc = sum;
@@ -203,86 +297,128 @@ __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uin
         const uint32_t g = lane * per + i;
         if (g >= p.groups) break;
         cum[g] = base;
-        base += (row1[g] - row0[g] + kBM - 1) / kBM;
+        base += (row1[g] - row0[g] + ROWS - 1) / ROWS;
     }
     if (lane == 31) cum[p.groups] = inc;
 }
 
-// A thread's run of 64 columns [c, c + 64) of row m.
-__device__ __forceinline__ void store_run(const Params &p, const uint64_t *acc, uint32_t m, uint32_t c)
+// ---- epilogue: 32 rows x 64 bytes of a warp through shared memory (2 KB, 16-byte units
+// rotated by the row), so that a store instruction covers eight whole 64-byte row
+// segments instead of 32 rows' 16 bytes.
+__device__ __forceinline__ void stage_put(uint8_t *buf, uint32_t lane, uint32_t j, uint4 v)
 {
-    const size_t at = (size_t)m * p.N + c;
-    if (p.out_f16) {
-        __half *o = static_cast<__half *>(p.out) + at;
-        if (p.vec && c + 64 <= p.N) {
+    *reinterpret_cast<uint4 *>(buf + lane * 64 + ((j ^ (lane >> 1)) & 3u) * 16) = v;
+}
+
+__device__ __forceinline__ uint4 stage_get(const uint8_t *buf, uint32_t row, uint32_t j)
+{
+    return *reinterpret_cast<const uint4 *>(buf + row * 64 + ((j ^ (row >> 1)) & 3u) * 16);
+}
+
+// The staged 64 bytes of rows [m, m + 32) below m_end, at byte `off` of rows of `pitch` bytes.
+__device__ __forceinline__ void stage_out(const uint8_t *buf, uint32_t lane, uint8_t *out, size_t pitch, size_t off, uint32_t m, uint32_t m_end)
+{
+    __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                uint32_t w[4];
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t r = i * 8 + (lane >> 2), j = lane & 3;
+        const uint4 v = stage_get(buf, r, j);
+        if (m + r < m_end) *reinterpret_cast<uint4 *>(out + (size_t)(m + r) * pitch + off + j * 16) = v;
+    }
+    __syncwarp();
+}
+
+// A warp's 32 rows x 64 columns of C from column c: lane = row.
+__device__ __forceinline__ void store_run(const Params &p, const float *acc, uint8_t *buf, uint32_t lane, uint32_t m, uint32_t m_end, uint32_t c)
+{
+    const uint32_t size = p.out_f16 ? 2u : 4u;
+    if (p.vec && c + 64 <= p.N) {
+        uint8_t *out = static_cast<uint8_t *>(p.out);
+        const size_t pitch = (size_t)p.N * size;
+        if (p.out_f16) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float2 f = unpack2(acc[4 * i + q]);
-                    w[q] = half2_bits(f.x, f.y);
+            for (uint32_t h = 0; h < 2; ++h) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const float *v = acc + 32 * h + 8 * j;
+                    stage_put(buf, lane, j, make_uint4(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]), half2_bits(v[4], v[5]), half2_bits(v[6], v[7])));
                 }
-                reinterpret_cast<uint4 *>(o)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                stage_out(buf, lane, out, pitch, (size_t)(c + 32 * h) * 2, m, m_end);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float2 f = unpack2(acc[i]);
-                if (c + 2 * i < p.N) o[2 * i] = __float2half_rn(f.x);
-                if (c + 2 * i + 1 < p.N) o[2 * i + 1] = __float2half_rn(f.y);
+            for (uint32_t h = 0; h < 4; ++h) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const float *v = acc + 16 * h + 4 * j;
+                    stage_put(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+                }
+                stage_out(buf, lane, out, pitch, (size_t)(c + 16 * h) * 4, m, m_end);
             }
         }
-    } else {
-        float *o = static_cast<float *>(p.out) + at;
-        if (p.vec && c + 64 <= p.N) {
+        return;
+    }
+    // rows that do not start on 16 bytes, or the last columns: 16 columns at a time
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 f = unpack2(acc[2 * i]), h = unpack2(acc[2 * i + 1]);
-                reinterpret_cast<float4 *>(o)[i] = make_float4(f.x, f.y, h.x, h.y);
-            }
-        } else {
+    for (uint32_t h = 0; h < 4; ++h) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float2 f = unpack2(acc[i]);
-                if (c + 2 * i < p.N) o[2 * i] = f.x;
-                if (c + 2 * i + 1 < p.N) o[2 * i + 1] = f.y;
+        for (uint32_t j = 0; j < 4; ++j) {
+            const float *v = acc + 16 * h + 4 * j;
+            stage_put(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+        }
+        __syncwarp();
+        const uint32_t cc = lane & 15, col = c + 16 * h + cc;
+#pragma unroll 4
+        for (uint32_t i = 0; i < 16; ++i) {
+            const uint32_t r = 2 * i + (lane >> 4);
+            const float v = *reinterpret_cast<const float *>(buf + r * 64 + (((cc >> 2) ^ (r >> 1)) & 3u) * 16 + (cc & 3) * 4);
+            if (m + r < m_end && col < p.N) {
+                const size_t at = (size_t)(m + r) * p.N + col;
+                if (p.out_f16) static_cast<__half *>(p.out)[at] = __float2half_rn(v);
+                else static_cast<float *>(p.out)[at] = v;
             }
         }
+        __syncwarp();
     }
 }
 
-// SPLIT: one tile per cluster; the cluster's CTAs take equal ranges of K blocks
-// and add their fp32 partials in rank order through distributed shared memory
-// (few rows: the products of a weight stream alone would leave SMs idle).
-template <int BN, int AR, int E, bool SPLIT>
+// SPLIT adds the CTAs' fp32 partials in rank order through distributed shared memory
+// (few rows: one CTA a weight tile would leave SMs idle); nothing but C leaves the cluster.
+template <int BN, int AR, int E, int MODE>
 __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_constant__ Params p)
 {
-    using C = Cfg<BN, AR>;
+    using C = Cfg<BN, AR, MODE>;
     constexpr int S = C::kStages;
-    constexpr uint32_t kRuns = BN / 128;     // 64-column runs per promotion thread
+    constexpr uint32_t kRuns = C::kRuns;     // a promotion thread has 64 columns of each run
     constexpr uint32_t kCols = E == EPI_SWIGLU ? BN / 2 : BN;   // output columns per tile
-    extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // The kernel has no static shared memory, so the dynamic part starts on its alignment.
+    // Addresses are then constants: rounding the base up would cost the promotion warps
+    // a register pair for every array.
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if ((smem_u32(smem) & 1023u) != 0u) {
+        if (threadIdx.x == 0) report_error(p.err, kErrBounds, 0xF82);
+        return;
+    }
     uint8_t *sA = smem, *sB = smem + C::kOffB;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
-    uint64_t *full = bars, *empty = bars + S;
-    uint64_t *acc_full = bars + 2 * S, *acc_empty = bars + 2 * S + 2, *drain = bars + 2 * S + 4;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S + 5);
+    uint64_t *full = bars, *empty = bars + S, *acc_full = empty + S, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *amax_x = reinterpret_cast<float *>(smem + C::kOffAmax);
     uint32_t *cum = reinterpret_cast<uint32_t *>(smem + C::kOffGroups);
     uint32_t *row0 = cum + p.groups + 1, *row1 = row0 + p.groups;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = MODE == SINGLE ? 0u : cta_rank();
     if (threadIdx.x == 0) {
+        constexpr uint32_t kSides = MODE == PAIR ? 2 : 1;   // the even CTA's full / acc_empty count both CTAs
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], 1);
+            mbar_init(&full[s], kSides);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 8);
+            mbar_init(&acc_empty[b], 8 * kSides);
         }
         mbar_init(drain, 1);
         *abort = 0;
@@ -291,20 +427,29 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         tma_prefetch_desc(&p.tm_b0);
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, C::kTmemCols);
-        tmem_relinquish();
+        if constexpr (MODE == PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc(tmem_slot, C::kTmemCols);
+            tmem_relinquish();
+        }
     }
-    if (warp == 2) build_groups(p, cum, row0, row1, lane);
+    if (warp == 2) build_groups<C::kTileRows>(p, cum, row0, row1, lane);
     tc_fence_before();
     __syncthreads();
+    if constexpr (MODE == PAIR) cluster_sync();   // the peer's barriers are initialised before any remote arrive
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const Groups gr{cum, row0, row1};
 
-    // SPLIT: blockIdx.x = tile * cluster + rank; K blocks [k0, k1) of this CTA
-    uint32_t t0 = blockIdx.x, step = gridDim.x, k0 = 0, k1 = p.kb, rank = 0, parts = 1;
-    if constexpr (SPLIT) {
-        asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    // SPLIT: K blocks [k0, k1) of this CTA. Clusters walk the tiles.
+    uint32_t t0 = blockIdx.x, step = gridDim.x, k0 = 0, k1 = p.kb, parts = 1;
+    if constexpr (MODE == PAIR) {
+        t0 >>= 1;
+        step >>= 1;
+    }
+    if constexpr (MODE == SPLIT) {
         asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
         t0 = blockIdx.x / parts;
         step = gridDim.x / parts;
@@ -313,137 +458,169 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     }
     const uint32_t total = cum[p.groups] * p.n_tiles;
 
-    // BN = 256: 64 packed accumulators and 64 words in flight need more than the 168
-    // registers a thread is launched with: 128 * 56 + 256 * 224 = 384 * 168
+    // BN = 256: a promotion thread keeps 128 accumulators and 64 words in flight, more
+    // than the 168 registers it is launched with: 128 * 40 + 256 * 232 = 384 * 168.
     if (warp < 4) {
-        if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == 0) {
-            // ------------------------------------------------ TMA producer
-            uint32_t g = 0;
-            bool alive = true;
-            for (uint32_t t = t0; t < total && alive; t += step) {
-                const Tile tl = tile_at(p, gr, t, kCols);
-                const uint32_t rows = min(tl.m_end - tl.m0, kBM), boxes = (rows + kBoxRows - 1) / kBoxRows;
-                const int32_t b_row = (int32_t)(tl.g * p.N + tl.n0);
-                // the second 128 rows of B: the up weights, or the next columns (none behind the last)
-                const bool second = BN == 256 && (E == EPI_SWIGLU || tl.n0 + 128 < p.N);
-                const uint32_t bytes = boxes * kBoxBytes + (second ? 2 : 1) * kBTile;
-                for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
-                    const uint32_t st = g % S, ph = (g / S) & 1u;
-                    if (!warp_wait(&empty[st], ph ^ 1u, abort, p.err, 0xF01)) { alive = false; break; }
-                    if (elect_one_sync()) {
-                        mbar_arrive_expect_tx(&full[st], bytes);
-                        const int32_t kc = (int32_t)(kk * kBK);
-                        tma_load_2d(sB + st * C::kBStage, &p.tm_b0, kc, b_row, &full[st]);
-                        if (second) {
-                            if constexpr (E == EPI_SWIGLU)
-                                tma_load_2d(sB + st * C::kBStage + kBTile, &p.tm_b1, kc, b_row, &full[st]);
-                            else
-                                tma_load_2d(sB + st * C::kBStage + kBTile, &p.tm_b0, kc, b_row + 128, &full[st]);
-                        }
+      if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+      if (warp == 0) {
+        // ------------------------------------------------ TMA producer
+        uint32_t g = 0;
+        bool alive = true;
+        for (uint32_t t = t0; t < total && alive; t += step) {
+            const Tile tl = tile_at<C::kTileRows>(p, gr, t, kCols);
+            // this CTA's rows of the tile (none for the odd CTA of a short one)
+            const uint32_t m0 = tl.m0 + (MODE == PAIR ? rank * kBM : 0u);
+            const uint32_t rows = m0 < tl.m_end ? min(tl.m_end - m0, kBM) : 0u, boxes = (rows + kBoxRows - 1) / kBoxRows;
+            const int32_t b_row = (int32_t)(tl.g * p.N + tl.n0);
+            // the second run: the up weights, or the next 128 columns (none behind the last)
+            const bool two = kRuns == 2 && (E == EPI_SWIGLU || tl.n0 + 128 < p.N);
+            const bool first = MODE != PAIR || rank == 0, second = two && (MODE != PAIR || rank == 1);
+            const uint32_t bytes = boxes * kBoxBytes + (first ? kBTile : 0u) + (second ? kBTile : 0u);
+            const CUtensorMap *tm1 = E == EPI_SWIGLU ? &p.tm_b1 : &p.tm_b0;
+            const int32_t b_row1 = b_row + (E == EPI_SWIGLU ? 0 : 128);
+            for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
+                const uint32_t st = g % S, ph = (g / S) & 1u;
+                if (!wait_all(&empty[st], ph ^ 1u, abort, p.err, 0xF01)) { alive = false; break; }
+                if (elect_one_sync()) {
+                    const int32_t kc = (int32_t)(kk * kBK);
+                    uint8_t *dA = sA + st * C::kAStage, *dB = sB + st * C::kBStage;
+                    if constexpr (MODE == PAIR) {
+                        const uint32_t bar = peer_addr(&full[st], 0);
+                        arrive_expect_tx_cl(bar, bytes);
+                        if (first) tma_load_2d_pair(dB, &p.tm_b0, kc, b_row, bar);
+                        if (second) tma_load_2d_pair(dB, tm1, kc, b_row1, bar);
                         for (uint32_t i = 0; i < boxes; ++i)
-                            tma_load_2d(sA + st * C::kAStage + i * kBoxBytes, &p.tm_a, kc,
-                                        (int32_t)(tl.m0 + i * kBoxRows), &full[st]);
+                            tma_load_2d_pair(dA + i * kBoxBytes, &p.tm_a, kc, (int32_t)(m0 + i * kBoxRows), bar);
+                    } else {
+                        mbar_arrive_expect_tx(&full[st], bytes);
+                        tma_load_2d(dB, &p.tm_b0, kc, b_row, &full[st]);
+                        if (second) tma_load_2d(dB + kBTile, tm1, kc, b_row1, &full[st]);
+                        for (uint32_t i = 0; i < boxes; ++i)
+                            tma_load_2d(dA + i * kBoxBytes, &p.tm_a, kc, (int32_t)(m0 + i * kBoxRows), &full[st]);
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
-            // drain: no copy may still be landing when the CTA exits
+        }
+        // drain: no copy may still be landing when the CTA exits (PAIR: the even CTA's
+        // barriers count both CTAs' copies, and the odd one waits for it)
+        if (MODE != PAIR || rank == 0)
             for (uint32_t q = (g > (uint32_t)S ? g - S : 0); q < g; ++q)
                 mbar_wait(&full[q % S], (q / S) & 1u, nullptr, p.err, 0xF02);
-        } else if (warp == 1) {
-            // ------------------------------------------------ MMA issuer
-            uint32_t g = 0;
-            bool alive = true;
-            for (uint32_t t = t0; t < total && alive; t += step) {
-                for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
-                    const uint32_t st = g % S, ph = (g / S) & 1u, b = g & 1u;
-                    if (!warp_wait(&acc_empty[b], ((g >> 1) & 1u) ^ 1u, abort, p.err, 0xF03) ||
-                        !warp_wait(&full[st], ph, abort, p.err, 0xF04)) { alive = false; break; }
-                    tc_fence_after();
-                    if (elect_one_sync()) {
-                        const uint64_t ad = smem_desc_sw128(sA + st * C::kAStage);
-                        const uint64_t bd = smem_desc_sw128(sB + st * C::kBStage);
-    #pragma unroll
-                        for (uint32_t k = 0; k < kBK / 32; ++k)
-                            mma_f8(tmem + b * BN, ad + 2 * k, bd + 2 * k, p.idesc, k != 0u);
-                        mma_commit(&empty[st]);
-                        mma_commit(&acc_full[b]);
+      } else if (warp == 1 && (MODE != PAIR || rank == 0)) {
+        // ------------------------------------------------ MMA issuer
+        const uint64_t ad0 = smem_desc_sw128(sA), bd0 = smem_desc_sw128(sB);
+        uint32_t g = 0;
+        bool alive = true;
+        for (uint32_t t = t0; t < total && alive; t += step) {
+            for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
+                const uint32_t st = g % S, b = g & 1u;
+                const uint64_t ad = ad0 + st * (C::kAStage >> 4), bd = bd0 + st * (C::kBStage >> 4);
+                if (!wait_all(&full[st], (g / S) & 1u, abort, p.err, 0xF04) ||
+                    !wait_all(&acc_empty[b], ((g >> 1) & 1u) ^ 1u, abort, p.err, 0xF03)) { alive = false; break; }
+                tc_fence_after();
+                if (elect_one_sync()) {
+#pragma unroll
+                    for (uint32_t k = 0; k < kBK / 32; ++k) {
+                        if constexpr (MODE == PAIR) mma_f8_pair(tmem + b * BN, ad + 2 * k, bd + 2 * k, p.idesc, k != 0u);
+                        else mma_f8(tmem + b * BN, ad + 2 * k, bd + 2 * k, p.idesc, k != 0u);
                     }
-                    __syncwarp();
+                    if constexpr (MODE == PAIR) {
+                        commit_pair(&acc_full[b]);
+                        commit_pair(&empty[st]);
+                    } else {
+                        mma_commit(&acc_full[b]);
+                        mma_commit(&empty[st]);
+                    }
                 }
+                __syncwarp();
             }
-            if (elect_one_sync()) mma_commit(drain);
-            __syncwarp();
         }
+        if (elect_one_sync()) {
+            if constexpr (MODE == PAIR) commit_pair(drain);
+            else mma_commit(drain);
+        }
+        __syncwarp();
+      }
     } else {
-        if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        if constexpr (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         // ------------------------------------------------ promotion and epilogue
         const uint32_t quarter = warp & 3, half = (uint32_t)(warp - 4) >> 2;
         const uint32_t lane_base = (quarter * 32u) << 16;
-        uint32_t g = 0, n_done = 0;
+        uint8_t *buf = smem + C::kOffOut + (warp - 4) * 2048;
+        uint32_t g = 0;
         bool alive = true;
-        for (uint32_t t = t0; t < total && alive; t += step, ++n_done) {
-            const Tile tl = tile_at(p, gr, t, kCols);
-            const uint32_t m = tl.m0 + quarter * 32 + lane;
-            const bool live = tl.m0 + quarter * 32 < tl.m_end;   // this warp's rows exist
+        for (uint32_t t = t0; t < total && alive; t += step) {
+            const Tile tl = tile_at<C::kTileRows>(p, gr, t, kCols);
+            const uint32_t m_warp = tl.m0 + (MODE == PAIR ? rank * kBM : 0u) + quarter * 32, m = m_warp + lane;
+            const bool live = m_warp < tl.m_end;   // this warp has rows
             const bool row_ok = m < tl.m_end;
-            // the thread's runs of 64 accumulator columns: run r starts at col(r)
-            auto col = [&](uint32_t r) -> uint32_t { return E == EPI_SWIGLU ? r * 128 + half * 64 : half * (BN / 2) + r * 64; };
+            // run r: accumulator columns [64 half, + 64) of run r's 128
+            const uint32_t nblk = tl.n0 / 128, two = kRuns == 2 && (E == EPI_SWIGLU || nblk + 1 < p.nb) ? 1u : 0u;
             const float *sa = p.sa + (size_t)(row_ok ? m : tl.m0) * p.kb;
-            const float *sb[2];
-            if constexpr (E == EPI_SWIGLU) {
-                const size_t blk = ((size_t)tl.g * p.nb + tl.n0 / 128) * p.kb;
-                sb[0] = p.sb0 + blk;
-                sb[1] = p.sb1 + blk;
-            } else {
-                const uint32_t nblk = min((tl.n0 + col(0)) / 128, p.nb - 1);
-                sb[0] = sb[1] = p.sb0 + ((size_t)tl.g * p.nb + nblk) * p.kb;
-            }
-            uint64_t acc[kRuns * 32];
+            const float *sb0 = p.sb0 + ((size_t)tl.g * p.nb + nblk) * p.kb;
+            const float *sb1 = E == EPI_SWIGLU ? p.sb1 + ((size_t)tl.g * p.nb + nblk) * p.kb : sb0 + (size_t)two * p.kb;
+            float acc[kRuns * 64];
 #pragma unroll
-            for (uint32_t i = 0; i < kRuns * 32; ++i) acc[i] = 0ull;
-            // scales two blocks ahead: an L2 round trip is longer than one block's MMAs
-            float a0 = 0.0f, a1 = 0.0f, u0 = 0.0f, u1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
-            auto fetch = [&](uint32_t kk, float &a, float &u, float &w) {
-                if (live && kk < k1) {
-                    a = __ldg(sa + kk);
-                    u = __ldg(sb[0] + kk);
-                    if constexpr (E == EPI_SWIGLU) w = __ldg(sb[1] + kk);
-                }
-            };
-            fetch(k0, a0, u0, w0);
-            fetch(k0 + 1, a1, u1, w1);
-            for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
-                const uint32_t b = g & 1u;
-                float a2 = 0.0f, u2 = 0.0f, w2 = 0.0f;
-                fetch(kk + 2, a2, u2, w2);
-                if (!warp_wait(&acc_full[b], (g >> 1) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
-                tc_fence_after();
-                if (live) {
-                    const uint32_t base = tmem + lane_base + b * BN;
-                    const uint64_t s0 = pack2(a0 * u0), s1 = E == EPI_SWIGLU ? pack2(a0 * w0) : s0;
-                    uint32_t d0[32], d1[32];
-                    tmem_ld_32x32b_x32(base + col(0), d0);
-                    tmem_ld_wait32(d0);
-#pragma unroll
-                    for (uint32_t r = 0; r < kRuns; ++r) {
-                        tmem_ld_32x32b_x32(base + col(r) + 32, d1);
-                        promote32(acc + r * 32, d0, r ? s1 : s0);
-                        tmem_ld_wait32(d1);
-                        if (r + 1 < kRuns) tmem_ld_32x32b_x32(base + col(r + 1), d0);
-                        promote32(acc + r * 32 + 16, d1, r ? s1 : s0);
-                        if (r + 1 < kRuns) tmem_ld_wait32(d0);
-                    }
-                }
+            for (uint32_t i = 0; i < kRuns * 64; ++i) acc[i] = 0.0f;
+            // read out: the accumulator may be filled again
+            auto release = [&](uint32_t b) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[b]);
-                a0 = a1; u0 = u1; w0 = w1;
-                a1 = a2; u1 = u2; w1 = w2;
+                if (lane == 0) {
+                    if constexpr (MODE == PAIR) arrive_cl(peer_addr(&acc_empty[b], 0));
+                    else mbar_arrive(&acc_empty[b]);
+                }
+            };
+            if (live) {
+                // Scales a block ahead, in registers that the unrolled loop names in turn:
+                // moving them on would wait for the loads.
+                float a[2], u0[2], u1[2];
+                auto fetch = [&](uint32_t kk, uint32_t i) {
+                    if (kk < k1) {
+                        a[i] = __ldg(sa + kk);
+                        u0[i] = __ldg(sb0 + kk);
+                        if constexpr (kRuns == 2) u1[i] = __ldg(sb1 + kk);
+                    }
+                };
+                fetch(k0, 0);
+                for (uint32_t kq = k0; kq < k1 && alive; kq += 2) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        if (kq + i >= k1) break;
+                        fetch(kq + i + 1, i ^ 1u);
+                        const uint32_t b = g & 1u;
+                        if (!wait_all(&acc_full[b], (g >> 1) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
+                        ++g;
+                        tc_fence_after();
+                        const uint32_t base = tmem + lane_base + b * BN + half * 64;
+                        const float s0 = a[i] * u0[i], s1 = kRuns == 2 ? a[i] * u1[i] : s0;
+                        uint32_t d[32], e[32];
+                        tmem_ld_32x32b_x32(base, d);
+                        tmem_ld_32x32b_x32(base + 32, e);
+                        tmem_ld_wait32(d);
+                        tmem_ld_wait32(e);
+                        if constexpr (kRuns == 2) {
+                            promote32(acc, d, s0);
+                            promote32(acc + 32, e, s0);
+                            tmem_ld_32x32b_x32(base + 128, d);
+                            tmem_ld_32x32b_x32(base + 160, e);
+                            tmem_ld_wait32(d);
+                            tmem_ld_wait32(e);
+                        }
+                        release(b);
+                        promote32(acc + kRuns * 64 - 64, d, s1);
+                        promote32(acc + kRuns * 64 - 32, e, s1);
+                    }
+                }
+            } else {
+                for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
+                    if (!wait_all(&acc_full[g & 1u], (g >> 1) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
+                    release(g & 1u);
+                }
             }
             if (E != EPI_SWIGLU && !alive) break;
-            if constexpr (SPLIT) {
+            if constexpr (MODE == SPLIT) {
                 // every copy has landed and every MMA has completed: the ring is free.
                 // Partials [row][BN] fp32, 16-byte columns rotated by the row against bank conflicts.
                 float4 *part = reinterpret_cast<float4 *>(smem);
@@ -451,9 +628,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     const uint32_t r = quarter * 32 + lane;
 #pragma unroll
                     for (uint32_t i = 0; i < kRuns * 16; ++i) {
-                        const float2 x = unpack2(acc[2 * i]), y = unpack2(acc[2 * i + 1]);
-                        const uint32_t c4 = half * (BN / 8) + i;
-                        part[r * (BN / 4) + ((c4 + r) & (BN / 4 - 1))] = make_float4(x.x, x.y, y.x, y.y);
+                        const uint32_t c4 = half * 16 + i;
+                        part[r * (BN / 4) + ((c4 + r) & (BN / 4 - 1))] =
+                            make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
                     }
                 }
             } else if constexpr (E == EPI_SWIGLU) {
@@ -461,42 +638,38 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 // channels, which this thread shares with the other column half's
                 float vmax = 0.0f;
 #pragma unroll
-                for (uint32_t i = 0; i < 32; ++i) {
-                    const float2 gt = unpack2(acc[i]), up = unpack2(acc[32 + i]);
-                    float2 v;
-                    v.x = __fdividef(gt.x, 1.0f + __expf(-gt.x)) * up.x;
-                    v.y = __fdividef(gt.y, 1.0f + __expf(-gt.y)) * up.y;
-                    vmax = fmaxf(vmax, fmaxf(fabsf(v.x), fabsf(v.y)));
-                    asm("mov.b64 %0, {%1, %2};" : "=l"(acc[i]) : "f"(v.x), "f"(v.y));
+                for (uint32_t i = 0; i < 64; ++i) {
+                    acc[i] = __fdividef(acc[i], 1.0f + __expf(-acc[i])) * acc[64 + i];
+                    vmax = fmaxf(vmax, fabsf(acc[i]));
                 }
                 const uint32_t r = quarter * 32 + lane;
-                float *ax = amax_x + (n_done & 1u) * 256;   // the barrier of the tile in between orders its reuse
-                ax[half * 128 + r] = vmax;
+                amax_x[half * 128 + r] = vmax;
                 alive = !promo_any(!alive);                 // all warps go on, or none does
                 if (!alive) break;
+                vmax = fmaxf(amax_x[r], amax_x[128 + r]);
+                asm volatile("barrier.sync 1, %0;" ::"n"(kPromoThreads) : "memory");   // before the next tile's write
                 // below 1e-30 the group is zero for every output type; the floor keeps qmax / vmax finite
-                vmax = fminf(fmaxf(fmaxf(ax[r], ax[128 + r]), 1.0e-30f), 3.0e38f);
+                vmax = fminf(fmaxf(vmax, 1.0e-30f), 3.0e38f);
                 const float qmax = f8_max(p.out_fmt);
                 const float inv = __fdiv_rn(qmax, vmax);
-                if (row_ok) {
-                    uint4 *o = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.out) + (size_t)m * p.N + tl.n0 + half * 64);
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        uint32_t w[4];
+                for (uint32_t i = 0; i < 4; ++i) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (uint32_t q = 0; q < 4; ++q) {
-                            const float2 x = unpack2(acc[8 * i + 2 * q]), y = unpack2(acc[8 * i + 2 * q + 1]);
-                            w[q] = enc_f8x2(p.out_fmt, x.x * inv, x.y * inv) | enc_f8x2(p.out_fmt, y.x * inv, y.y * inv) << 16;
-                        }
-                        o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (uint32_t q = 0; q < 4; ++q) {
+                        const float *v = acc + 16 * i + 4 * q;
+                        w[q] = enc_f8x2(p.out_fmt, v[0] * inv, v[1] * inv) | enc_f8x2(p.out_fmt, v[2] * inv, v[3] * inv) << 16;
                     }
-                    if (half == 0)
-                        p.out_scales[(size_t)m * p.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
+                    stage_put(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
                 }
-            } else if (row_ok) {
+                stage_out(buf, lane, static_cast<uint8_t *>(p.out), p.N, tl.n0 + half * 64, m_warp, tl.m_end);
+                if (row_ok && half == 0) p.out_scales[(size_t)m * p.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
+            } else if (live) {
 #pragma unroll
-                for (uint32_t r = 0; r < kRuns; ++r)
-                    if (tl.n0 + col(r) < p.N) store_run(p, acc + r * 32, m, tl.n0 + col(r));
+                for (uint32_t r = 0; r < kRuns; ++r) {
+                    const uint32_t c = tl.n0 + r * 128 + half * 64;
+                    if (c < p.N) store_run(p, acc + r * 64, buf, lane, m_warp, tl.m_end, c);
+                }
             }
         }
     }
@@ -504,15 +677,20 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     // ---------------------------------------------------- teardown
     tc_fence_before();
     __syncthreads();
+    if (warp == 1 && (MODE != PAIR || rank == 0)) mbar_wait(drain, 0, nullptr, p.err, 0xF06);   // every issued MMA has completed
+    __syncthreads();
+    // PAIR: neither CTA leaves while the other arrives on its barriers or the MMAs
+    // read its memory. SPLIT: the partials are complete.
+    if constexpr (MODE != SINGLE) cluster_sync();
     if (warp == 1) {
-        mbar_wait(drain, 0, nullptr, p.err, 0xF06);   // every issued MMA has completed
         tc_fence_after();
-        tmem_dealloc(tmem, C::kTmemCols);
+        if constexpr (MODE == PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
+        else tmem_dealloc(tmem, C::kTmemCols);
     }
-    if constexpr (SPLIT) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if constexpr (MODE == SPLIT) {
         if (t0 < total && !*abort) {
-            const Tile tl = tile_at(p, gr, t0, kCols);
+            const Tile tl = tile_at<C::kTileRows>(p, gr, t0, kCols);
             const uint32_t rows = min(tl.m_end - tl.m0, kBM), base = smem_u32(smem);
             // the cluster's CTAs take every parts-th 16-byte column of the tile, summed in rank order
             for (uint32_t i = threadIdx.x * parts + rank; i < rows * (BN / 4); i += kThreads * parts) {
@@ -554,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             }
         }
         // a peer may still be reading this CTA's partials
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_sync();
     }
 }
 
