@@ -10,8 +10,16 @@
 // (and without sums of two scores) v is monotone in the logit, so the logits are
 // compared themselves. Otherwise fp32 scores decide, and wherever two values that
 // the outcome depends on lie closer than the fp32 error, that warp computes the
-// token again in 64 bits: about one token in a thousand for scores of a trained
-// router's spread, which costs less than 64-bit exponentials for all of them.
+// token again in 64 bits (exact_token): a few tokens in a thousand for scores of a
+// trained router's spread, which costs less than 64-bit exponentials for all.
+//
+// fast_kernel: a lane holds PER neighbouring experts (16-byte loads), sorted once by
+// 32-bit keys that carry the position in their lowest bits; each of the k rounds is
+// then one warp-wide maximum of the lanes' heads and a shift in the winner's lane.
+// A group is a run of lanes, its two best a butterfly. 32768 tokens of 256 experts are
+// bound by instruction issue, not by the 34 MB they read.
+// any_kernel (every token through the exact comparison in fp32, then 64 bits where
+// needed) takes the group sizes that do not fall on lane borders.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -33,6 +41,7 @@ struct Params {
     float *weights;         // [T][k]
     uint32_t T, E, k, groups, top_groups, group_top, group_size;
     int sigmoid, renorm, f16, by_logit;   // by_logit: v is the logit
+    int vec;                              // rows of logits start on 16 bytes
     float scale;
 };
 
@@ -69,7 +78,7 @@ template <typename F> __device__ __forceinline__ F warp_max(F v)
     return v;
 }
 
-// The token's chosen experts: lane s < k gets the expert of slot s. Returns whether
+// Exact comparisons in layout expert = lane + 32 j. The token's chosen experts: lane s < k gets the expert of slot s. Returns whether
 // the choice holds for the exact values (always for F = double).
 template <typename F, int PER>
 __device__ __forceinline__ bool choose(const Params &p, const float (&z)[PER], uint32_t lane, F *sv, uint32_t &mine)
@@ -185,24 +194,25 @@ __device__ __forceinline__ bool choose(const Params &p, const float (&z)[PER], u
     return sure;
 }
 
+// One token decided exactly; sv: E doubles of shared memory where groups are dropped.
 template <int PER>
-__global__ void __launch_bounds__(32 * kWarps) gate_kernel(const Params p)
+__device__ __noinline__ uint32_t exact_token(const Params &p, size_t row, uint32_t lane, double *sv)
 {
-    extern __shared__ double smem[];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double *sv = smem + (size_t)warp * p.E;
-    const uint32_t t = blockIdx.x * kWarps + warp;
-    if (t >= p.T) return;
-    const size_t row = (size_t)t * p.E;
     float z[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) z[j] = lane + 32 * j < p.E ? load_logit(p, row + lane + 32 * j) : -INFINITY;
     uint32_t e = 0;
-    if (!choose<float, PER>(p, z, lane, reinterpret_cast<float *>(sv), e)) choose<double, PER>(p, z, lane, sv, e);
+    if (!p.by_logit || !choose<float, PER>(p, z, lane, reinterpret_cast<float *>(sv), e)) choose<double, PER>(p, z, lane, sv, e);
+    return e;
+}
 
-    // weights of the chosen: lane s has slot s
+// Weight of the lane's chosen expert e (lanes below k). zmax and zsum: softmax's
+// maximum and sum over all experts, used without renormalisation.
+__device__ __forceinline__ void write_slot(const Params &p, size_t t, uint32_t lane, uint32_t e, float zmax, float zsum)
+{
     const bool have = lane < p.k;
-    float zc = have ? load_logit(p, row + e) : -INFINITY, w = 0.0f, sum;
+    const float zc = have ? load_logit(p, t * p.E + e) : -INFINITY;
+    float w = 0.0f, sum;
     if (p.renorm) {
         // relative to the largest chosen logit, so that scores too small for fp32 keep their ratio
         const float m = warp_max(zc);
@@ -218,21 +228,252 @@ __global__ void __launch_bounds__(32 * kWarps) gate_kernel(const Params p)
         w = __fdiv_rn(1.0f, 1.0f + expf(-zc));
         sum = 1.0f;
     } else {
-        float m = z[0];
-#pragma unroll
-        for (int j = 1; j < PER; ++j) m = fmaxf(m, z[j]);
-        m = warp_max(m);
-        sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) sum += z[j] > -INFINITY ? (z[j] == m ? 1.0f : expf(z[j] - m)) : 0.0f;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-        if (zc > -INFINITY) w = zc == m ? 1.0f : expf(zc - m);
+        if (zc > -INFINITY) w = zc == zmax ? 1.0f : expf(zc - zmax);
+        sum = zsum;
     }
     if (have) {
-        p.ids[(size_t)t * p.k + lane] = (int32_t)e;
-        p.weights[(size_t)t * p.k + lane] = sum > 0.0f ? __fdiv_rn(w, sum) * p.scale : 0.0f;
+        p.ids[t * p.k + lane] = (int32_t)e;
+        p.weights[t * p.k + lane] = sum > 0.0f ? __fdiv_rn(w, sum) * p.scale : 0.0f;
     }
+}
+
+// Softmax's maximum and sum (accurate exponentials) over the lanes' z.
+template <int PER> __device__ __forceinline__ void softmax_norm(const float (&z)[PER], float &m, float &sum)
+{
+    m = z[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) m = fmaxf(m, z[j]);
+    m = warp_max(m);
+    sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += z[j] > -INFINITY ? (z[j] == m ? 1.0f : expf(z[j] - m)) : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+}
+
+template <int PER>
+__global__ void __launch_bounds__(32 * kWarps) any_kernel(const Params p)
+{
+    extern __shared__ double smem[];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double *sv = smem + (size_t)warp * p.E;
+    const uint32_t t = blockIdx.x * kWarps + warp;
+    if (t >= p.T) return;
+    const size_t row = (size_t)t * p.E;
+    float z[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) z[j] = lane + 32 * j < p.E ? load_logit(p, row + lane + 32 * j) : -INFINITY;
+    uint32_t e = 0;
+    if (!choose<float, PER>(p, z, lane, reinterpret_cast<float *>(sv), e)) choose<double, PER>(p, z, lane, sv, e);
+    float m = 0.0f, sum = 1.0f;
+    if (!p.renorm && !p.sigmoid) softmax_norm<PER>(z, m, sum);
+    write_slot(p, t, lane, e, m, sum);
+}
+
+// Order-preserving bits of a float (not NaN); never 0.
+__device__ __forceinline__ uint32_t order_bits(float v)
+{
+    const uint32_t u = __float_as_uint(v);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__device__ __forceinline__ float order_value(uint32_t k)
+{
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+
+__host__ __device__ constexpr int key_bits(int per) { return per <= 1 ? 0 : per <= 2 ? 1 : per <= 4 ? 2 : per <= 8 ? 3 : 4; }
+
+// Batcher's odd-even merge sort, descending, of any N (comparators beyond N are left out).
+template <int N> __device__ __forceinline__ void sort_desc(uint32_t (&k)[N])
+{
+#pragma unroll
+    for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+        for (int q = p; q >= 1; q >>= 1)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t a = k[i + j], b = k[i + j + q];
+                        k[i + j] = max(a, b);
+                        k[i + j + q] = min(a, b);
+                    }
+}
+
+template <int PER, bool F16>
+__device__ __forceinline__ void load_lane(const Params &p, uint32_t t, uint32_t lane, float (&z)[PER])
+{
+    const size_t at = (size_t)t * p.E + lane * PER;
+    if (PER % 4 == 0 && p.vec && p.E % PER == 0) {   // whole lanes, on 8 bytes at least
+        const bool have = lane * PER < p.E;
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j) {
+            float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (have) {
+                if (F16) {
+                    const uint2 h = __ldg(reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.logits) + at) + j);
+                    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h.x));
+                    const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h.y));
+                    v = make_float4(a.x, a.y, b.x, b.y);
+                } else {
+                    v = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.logits) + at) + j);
+                }
+            }
+            z[4 * j] = v.x; z[4 * j + 1] = v.y; z[4 * j + 2] = v.z; z[4 * j + 3] = v.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        z[j] = -INFINITY;
+        if (lane * PER + j < p.E)
+            z[j] = F16 ? __half2float(static_cast<const __half *>(p.logits)[at + j]) : static_cast<const float *>(p.logits)[at + j];
+    }
+}
+
+// group_lanes: lanes a group takes (a
+// power of two) where groups are dropped, else 0.
+template <int PER, bool F16>
+__global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint32_t group_lanes)
+{
+    extern __shared__ double smem[];
+    __shared__ uint32_t sel[kWarps][32];
+    constexpr int kBits = key_bits(PER);
+    constexpr uint32_t kLow = (1u << kBits) - 1u;
+    constexpr int kExactPer = PER <= 2 ? 2 : PER <= 4 ? 4 : PER <= 8 ? 8 : 16;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double *sv = smem + (size_t)warp * p.E;
+    const uint32_t stride = gridDim.x * kWarps;
+    uint32_t t = blockIdx.x * kWarps + warp;
+    if (t >= p.T) return;
+    float bias[PER], zn[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) bias[j] = p.bias && lane * PER + j < p.E ? p.bias[lane * PER + j] : 0.0f;
+    load_lane<PER, F16>(p, t, lane, zn);
+    // what two compared values may be off by together, beside the keys' cut bits:
+    // fp32 scores, or nothing where the logits are compared
+    const float tol = p.by_logit ? 0.0f : p.sigmoid ? 1.0f / 1048576.0f : 1.0f / 262144.0f;
+    const float cut = (float)(2u << kBits) / 8388608.0f;
+    const bool check = !(p.by_logit && F16);   // fp16 logits lose no bits to the position
+    for (; t < p.T; t += stride) {
+        float z[PER], v[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) z[j] = zn[j] > -INFINITY ? zn[j] + 0.0f : -INFINITY;   // NaN masks; -0 -> +0
+        if (t + stride < p.T) load_lane<PER, F16>(p, t + stride, lane, zn);
+        float zm = 0.0f, zsum = 1.0f;
+        if (p.by_logit) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] = z[j];
+        } else {
+            if (p.sigmoid) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) v[j] = Num<float>::rcp(1.0f + Num<float>::exp(-z[j]));
+            } else {
+                zm = z[0];
+#pragma unroll
+                for (int j = 1; j < PER; ++j) zm = fmaxf(zm, z[j]);
+                zm = warp_max(zm);
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    v[j] = z[j] == zm ? 1.0f : Num<float>::exp(z[j] - zm);
+                    if (!(z[j] > -INFINITY)) v[j] = 0.0f;
+                    sum += v[j];
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+                const float r = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) v[j] *= r;
+            }
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                v[j] += bias[j];
+                v[j] = z[j] > -INFINITY && v[j] > -INFINITY ? v[j] + 0.0f : -INFINITY;   // NaN too
+            }
+        }
+        bool sure = true, keep = lane * PER < p.E;
+        if (group_lanes) {
+            float b0 = v[0], b1 = -INFINITY;
+#pragma unroll
+            for (int j = 1; j < PER; ++j) {
+                b1 = fmaxf(b1, fminf(b0, v[j]));
+                b0 = fmaxf(b0, v[j]);
+            }
+            for (uint32_t o = group_lanes >> 1; o; o >>= 1) {
+                const float o0 = __shfl_xor_sync(kFull, b0, o), o1 = __shfl_xor_sync(kFull, b1, o);
+                b1 = fmaxf(fminf(b0, o0), fmaxf(b1, o1));
+                b0 = fmaxf(b0, o0);
+            }
+            const float worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
+            const uint32_t mine = lane / group_lanes;
+            uint32_t rank = 0;
+            for (uint32_t g = 0; g < p.groups; ++g) {
+                const float w = __shfl_sync(kFull, worth, g * group_lanes);
+                rank += w > worth || (w == worth && g < mine) ? 1u : 0u;
+            }
+            const bool real = mine < p.groups;
+            keep = real && rank < p.top_groups;
+            if (!p.by_logit) {
+                // the last group that stays and the first that goes have to be well apart
+                const uint32_t k = order_bits(worth);
+                const float in = order_value(__reduce_min_sync(kFull, keep ? k : 0xFFFFFFFFu));
+                const float out = order_value(__reduce_max_sync(kFull, real && !keep ? k : 0u));
+                sure = in - out > 2.0f * tol * (1.0f + fabsf(in));
+            }
+        }
+        uint32_t key[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            key[j] = keep && lane * PER + j < p.E ? (order_bits(v[j]) & ~kLow) | (kLow - (uint32_t)j) : 0u;
+        sort_desc<PER>(key);
+        uint32_t won = 0;   // lane s: the winning key of round s
+        for (uint32_t s = 0; s < p.k; ++s) {
+            const uint32_t m = __reduce_max_sync(kFull, key[0]);
+            // equal but for the position: the lowest lane has the lowest expert
+            const uint32_t first = __ffs(__ballot_sync(kFull, (key[0] >> kBits) == (m >> kBits))) - 1;
+            if (lane == s) won = m;
+            if (lane == first) {
+                sel[warp][s] = lane * PER + (kLow - (key[0] & kLow));
+#pragma unroll
+                for (int j = 0; j + 1 < PER; ++j) key[j] = key[j + 1];
+                key[PER - 1] = 0u;
+            }
+        }
+        if (check) {
+            // neighbours in the order, the first not chosen among them, have to be apart
+            const uint32_t after = __reduce_max_sync(kFull, key[0]);
+            uint32_t next = __shfl_down_sync(kFull, won, 1);
+            if (lane + 1 == p.k) next = after;
+            if (lane < p.k && next != 0u) {
+                const float a = order_value(won | kLow), b = order_value(next | kLow);
+                sure = sure && a - b > 2.0f * tol + fmaxf(fabsf(a), fabsf(b)) * (cut + 2.0f * tol);
+            }
+        }
+        __syncwarp();
+        uint32_t e = lane < p.k ? sel[warp][lane] : 0u;
+        if (!__all_sync(kFull, sure)) e = exact_token<kExactPer>(p, (size_t)t * p.E, lane, sv);
+        if (!p.renorm && !p.sigmoid) softmax_norm<PER>(z, zm, zsum);
+        write_slot(p, t, lane, e, zm, zsum);
+        __syncwarp();
+    }
+}
+
+template <bool F16> cudaError_t launch_fast(const Params &p, uint32_t per, uint32_t group_lanes, cudaStream_t st)
+{
+    // a warp keeps bias and the next token's logits in registers: no more CTAs than run at once
+    const uint32_t want = (p.T + kWarps - 1) / kWarps, most = 148 * 8;
+    const unsigned grid = want < most ? want : most;
+    const size_t smem = group_lanes ? (size_t)kWarps * p.E * sizeof(double) : 0;
+    switch (per) {
+#define GATE_CASE(N) case N: fast_kernel<N, F16><<<grid, 32 * kWarps, smem, st>>>(p, group_lanes); break;
+    GATE_CASE(1) GATE_CASE(2) GATE_CASE(3) GATE_CASE(4) GATE_CASE(5) GATE_CASE(6) GATE_CASE(8) GATE_CASE(10) GATE_CASE(12)
+    GATE_CASE(16)
+#undef GATE_CASE
+    }
+    return cudaGetLastError();
 }
 
 }  // namespace gate
@@ -249,12 +490,22 @@ cudaError_t launch_moe_gate(const GateLaunch &L, cudaStream_t st)
     // one score's order is its logit's; only a bias or a sum of two needs the scores
     p.by_logit = !L.bias && (L.top_groups == L.groups || L.group_top == 1 || p.group_size == 1);
     p.scale = L.scale;
+    p.vec = (size_t)L.E * (L.f16 ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(L.logits) & 15u) == 0;
+    const bool grouped = L.top_groups < L.groups;
+    // experts a lane: the fewest that hold all, and a group in a power of two of lanes
+    for (uint32_t per : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 10u, 12u, 16u}) {
+        if (per * 32 < L.E) continue;
+        if (!grouped) return L.f16 ? launch_fast<true>(p, per, 0, st) : launch_fast<false>(p, per, 0, st);
+        const uint32_t lanes = p.group_size / per;
+        if (p.group_size % per || (lanes & (lanes - 1))) continue;
+        return L.f16 ? launch_fast<true>(p, per, lanes, st) : launch_fast<false>(p, per, lanes, st);
+    }
     const unsigned grid = (L.T + kWarps - 1) / kWarps;
-    const size_t smem = L.top_groups < L.groups ? (size_t)kWarps * L.E * sizeof(double) : 0;
-    if (L.E <= 64) gate_kernel<2><<<grid, 32 * kWarps, smem, st>>>(p);
-    else if (L.E <= 128) gate_kernel<4><<<grid, 32 * kWarps, smem, st>>>(p);
-    else if (L.E <= 256) gate_kernel<8><<<grid, 32 * kWarps, smem, st>>>(p);
-    else gate_kernel<16><<<grid, 32 * kWarps, smem, st>>>(p);
+    const size_t smem = (size_t)kWarps * L.E * sizeof(double);
+    if (L.E <= 64) any_kernel<2><<<grid, 32 * kWarps, smem, st>>>(p);
+    else if (L.E <= 128) any_kernel<4><<<grid, 32 * kWarps, smem, st>>>(p);
+    else if (L.E <= 256) any_kernel<8><<<grid, 32 * kWarps, smem, st>>>(p);
+    else any_kernel<16><<<grid, 32 * kWarps, smem, st>>>(p);
     return cudaGetLastError();
 }
 
