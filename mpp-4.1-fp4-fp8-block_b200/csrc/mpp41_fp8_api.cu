@@ -162,28 +162,29 @@ mpp41_status mpp41_matmul_fp8_grouped(mpp41_ctx *ctx, int a_fmt, const void *a, 
 namespace {
 
 struct MoeFp8Layout {
-    size_t offsets, inv, pq, ps, mq, ms, y, xq, xs, smq, sms, sy, total;
+    size_t offsets, inv, rw, pq, ps, mq, ms, y, xq, xs, smq, sms, sy, total;
 };
 
 MoeFp8Layout moe_fp8_layout(const mpp41_moe_fp8_desc *d)
 {
     const size_t T = d->tokens, H = d->hidden, I = d->intermediate, R = T * d->top_k, Is = d->shared_intermediate;
-    const size_t Ts = Is ? T : 0;
+    const size_t Ts = Is ? T : 0, out_size = d->out_f16 ? 2 : 4;
     MoeFp8Layout l;
     size_t o = 0;
     auto part = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
     l.offsets = part((d->experts + (size_t)1) * 4);
     l.inv = part(R * 4);
+    l.rw = part(R * 4);
     l.pq = part(R * H);
     l.ps = part(R * (H / 128) * 4);
     l.mq = part(R * I);
     l.ms = part(R * (I / 128) * 4);
-    l.y = part(R * H * 4);
+    l.y = part(R * H * out_size);
     l.xq = part(Ts * H);
     l.xs = part(Ts * (H / 128) * 4);
     l.smq = part(Ts * Is);
     l.sms = part(Ts * (Is / 128) * 4);
-    l.sy = part(Ts * H * 4);
+    l.sy = part(Ts * H * out_size);
     l.total = o;
     return l;
 }
@@ -238,12 +239,12 @@ mpp41_status mpp41_moe_fp8(mpp41_ctx *ctx, const mpp41_moe_fp8_desc *d, const vo
     auto f32 = [&](size_t at) { return reinterpret_cast<float *>(b + at); };
     int32_t *offsets = reinterpret_cast<int32_t *>(b + l.offsets), *inv = reinterpret_cast<int32_t *>(b + l.inv);
     cudaStream_t st = ctx->stream;
-    s = cuda_status(launch_fp8_plan(ids, R, E, offsets, inv, ctx->err, st), "plan");
+    s = cuda_status(launch_fp8_plan(ids, weights, R, E, offsets, inv, f32(l.rw), ctx->err, st), "plan");
     if (s != MPP41_OK) return s;
     s = cuda_status(launch_fp8_scatter(d->fmt, x, T, H, inv, k, b + l.pq, f32(l.ps), Is ? b + l.xq : nullptr,
                                        Is ? f32(l.xs) : nullptr, st), "quantize x");
     if (s != MPP41_OK) return s;
-    Fp8Launch g{};
+    Fp8Launch g{}, gs{}, n{}, ns{};
     g.a = b + l.pq; g.sa = f32(l.ps);
     g.b0 = wg; g.sb0 = sg; g.b1 = wu; g.sb1 = su;
     g.offsets = offsets; g.groups = E;
@@ -251,36 +252,34 @@ mpp41_status mpp41_moe_fp8(mpp41_ctx *ctx, const mpp41_moe_fp8_desc *d, const vo
     g.M = R; g.N = I; g.K = H;
     g.a_fmt = g.b_fmt = g.out_fmt = d->fmt;
     g.err = ctx->err;
+    n = g;
+    n.a = b + l.mq; n.sa = f32(l.ms);
+    n.b0 = wd; n.sb0 = sd; n.b1 = nullptr; n.sb1 = nullptr;
+    n.out = b + l.y; n.out_scales = nullptr;
+    n.row_scale = f32(l.rw);
+    n.N = H; n.K = I;
+    n.out_f16 = d->out_f16 != 0;
+    if (Is) {
+        gs = g;
+        gs.a = b + l.xq; gs.sa = f32(l.xs);
+        gs.b0 = shared_wg; gs.sb0 = shared_sg; gs.b1 = shared_wu; gs.sb1 = shared_su;
+        gs.offsets = nullptr; gs.groups = 1;
+        gs.out = b + l.smq; gs.out_scales = f32(l.sms);
+        gs.M = T; gs.N = Is;
+        ns = n;
+        ns.a = b + l.smq; ns.sa = f32(l.sms);
+        ns.b0 = shared_wd; ns.sb0 = shared_sd;
+        ns.offsets = nullptr; ns.groups = 1;
+        ns.out = b + l.sy; ns.row_scale = nullptr;
+        ns.M = T; ns.K = Is;
+        g.more = &gs;
+        n.more = &ns;
+    }
     s = run_gemm(g, st, "expert gate/up product");
     if (s != MPP41_OK) return s;
-    Fp8Launch n{};
-    n.a = b + l.mq; n.sa = f32(l.ms);
-    n.b0 = wd; n.sb0 = sd;
-    n.offsets = offsets; n.groups = E;
-    n.out = b + l.y;
-    n.M = R; n.N = H; n.K = I;
-    n.a_fmt = n.b_fmt = d->fmt;
-    n.err = ctx->err;
     s = run_gemm(n, st, "expert down product");
     if (s != MPP41_OK) return s;
-    if (Is) {
-        g.a = b + l.xq; g.sa = f32(l.xs);
-        g.b0 = shared_wg; g.sb0 = shared_sg; g.b1 = shared_wu; g.sb1 = shared_su;
-        g.offsets = nullptr; g.groups = 1;
-        g.out = b + l.smq; g.out_scales = f32(l.sms);
-        g.M = T; g.N = Is;
-        s = run_gemm(g, st, "shared expert gate/up product");
-        if (s != MPP41_OK) return s;
-        n.a = b + l.smq; n.sa = f32(l.sms);
-        n.b0 = shared_wd; n.sb0 = shared_sd;
-        n.offsets = nullptr; n.groups = 1;
-        n.out = b + l.sy;
-        n.M = T; n.K = Is;
-        s = run_gemm(n, st, "shared expert down product");
-        if (s != MPP41_OK) return s;
-    }
-    return cuda_status(launch_fp8_combine(f32(l.y), inv, weights, T, k, H, Is ? f32(l.sy) : nullptr, out, d->out_f16 != 0, st),
-                       "combine");
+    return cuda_status(launch_fp8_combine(b + l.y, inv, T, k, H, Is ? b + l.sy : nullptr, out, d->out_f16 != 0, st), "combine");
 }
 
 }  // extern "C"

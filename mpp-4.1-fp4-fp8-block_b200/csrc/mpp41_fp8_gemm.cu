@@ -32,7 +32,7 @@ template <int BN, int AR, int E, int MODE> cudaError_t prepare(int dev)
     static std::atomic<uint64_t> done;
     if (done.load(std::memory_order_acquire) >> dev & 1u) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<BN, AR, E, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)(Cfg<BN, AR, MODE>::kSmem + 4 * (3 * kFp8MaxGroups + 1)));
+                                               (int)(Cfg<BN, AR, MODE>::kSmem + group_bytes(kFp8MaxGroups + 1)));
     if (e == cudaSuccess) done.fetch_or(1ull << dev, std::memory_order_release);
     return e;
 }
@@ -51,7 +51,7 @@ template <int BN, int AR> int resident_clusters(int dev, int parts)
         at.val.clusterDim.y = at.val.clusterDim.z = 1;
         cfg.gridDim = dim3((unsigned)parts);
         cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = Cfg<BN, AR, SPLIT>::kSmem + 4 * 4;
+        cfg.dynamicSmemBytes = Cfg<BN, AR, SPLIT>::kSmem + group_bytes(1);
         cfg.attrs = &at;
         cfg.numAttrs = 1;
         if (cudaOccupancyMaxActiveClusters(&v, fp8_gemm_kernel<BN, AR, EPI_STORE, SPLIT>, &cfg) != cudaSuccess) {
@@ -76,7 +76,7 @@ cudaError_t launch(const Params &p, int dev, uint32_t grid, uint32_t parts, cuda
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Cfg<BN, AR, MODE>::kSmem + 4 * (3 * p.groups + 1);
+    cfg.dynamicSmemBytes = Cfg<BN, AR, MODE>::kSmem + group_bytes(p.all_groups);
     cfg.stream = st;
     cfg.attrs = &at;
     cfg.numAttrs = MODE == SINGLE ? 0 : 1;
@@ -86,64 +86,76 @@ cudaError_t launch(const Params &p, int dev, uint32_t grid, uint32_t parts, cuda
 }  // namespace
 }  // namespace fp8
 
+namespace {
+
+// One side's fields; false when a tensor map cannot be made.
+bool fill(fp8::Side &d, const Fp8Launch &L, uint32_t cols)
+{
+    using namespace fp8;
+    const bool swiglu = L.b1 != nullptr;
+    d.sa = L.sa; d.sb0 = L.sb0; d.sb1 = L.sb1;
+    d.out = L.out; d.out_scales = L.out_scales; d.row_scale = L.row_scale;
+    d.M = L.M; d.N = L.N;
+    d.kb = (L.K + kBK - 1) / kBK;
+    d.nb = (L.N + 127) / 128;
+    d.n_tiles = (L.N + cols - 1) / cols;
+    const size_t row = (size_t)L.N * (swiglu ? 1 : L.out_f16 ? 2 : 4);
+    d.vec = row % 16 == 0 && (reinterpret_cast<uintptr_t>(L.out) & 15u) == 0;
+    const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const uint64_t b_rows = (uint64_t)L.groups * L.N;
+    return make_map(&d.tm_a, L.a, u8, 1, L.K, L.M, kBK, kBoxRows, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           make_map(&d.tm_b0, L.b0, u8, 1, L.K, b_rows, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B) &&
+           (!swiglu || make_map(&d.tm_b1, L.b1, u8, 1, L.K, b_rows, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B));
+}
+
+}  // namespace
+
 int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
 {
     using namespace fp8;
     const bool swiglu = L.b1 != nullptr;
-    if (!L.M || !L.N || !L.groups) return 0;
+    const Fp8Launch *more = L.more && L.more->M && L.more->N ? L.more : nullptr;
+    if (!L.M || !L.N || !L.groups) return more ? launch_fp8_gemm(*more, st, why) : 0;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || dev >= kMaxDevices) { *why = "device"; return 2; }
-    Params p;
-    memset(&p, 0, sizeof(p));
-    p.sa = L.sa; p.sb0 = L.sb0; p.sb1 = L.sb1;
-    p.offsets = L.offsets;
-    p.out = L.out; p.out_scales = L.out_scales;
-    p.M = L.M; p.N = L.N; p.K = L.K;
-    p.kb = (L.K + kBK - 1) / kBK;
-    p.nb = (L.N + 127) / 128;
-    p.groups = L.groups;
-    p.out_f16 = L.out_f16;
-    p.out_fmt = L.out_fmt;
-    const size_t row = (size_t)L.N * (swiglu ? 1 : L.out_f16 ? 2 : 4);
-    p.vec = row % 16 == 0 && (reinterpret_cast<uintptr_t>(L.out) & 15u) == 0;
-    p.err = L.err;
     // Row tiles at most (a group's last may be partial), of 128 rows and of a pair's 256.
     // Pairs where groups fill more than one row tile on average: the half of a pair that
     // has no rows would only move weights.
     const uint64_t mt = L.offsets ? L.M / kBM + (L.groups < L.M ? L.groups : L.M) : (L.M + kBM - 1) / kBM;
     const uint64_t sms = (uint64_t)sm_count(dev);
-    const bool few = !swiglu && !L.offsets && mt * ((L.N + 255) / 256) < sms && mt * ((L.N + 127) / 128) <= sms;
+    const bool few = !swiglu && !L.offsets && !more && mt * ((L.N + 255) / 256) < sms && mt * ((L.N + 127) / 128) <= sms;
     const bool pair = !few && L.M / L.groups > 128;
-    const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const uint64_t b_rows = (uint64_t)L.groups * L.N;
-    if (!make_map(&p.tm_a, L.a, u8, 1, L.K, L.M, kBK, kBoxRows, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !make_map(&p.tm_b0, L.b0, u8, 1, L.K, b_rows, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        (swiglu && !make_map(&p.tm_b1, L.b1, u8, 1, L.K, b_rows, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B))) {
-        *why = "tensor maps";
-        return 2;
-    }
+    const uint32_t cols = swiglu || few ? 128 : 256;
+    Params p;
+    memset(&p, 0, sizeof(p));
+    if (!fill(p.side[0], L, cols) || (more && !fill(p.side[1], *more, cols))) { *why = "tensor maps"; return 2; }
+    p.offsets = L.offsets;
+    p.groups = L.groups;
+    p.all_groups = L.groups + (more ? 1 : 0);
+    p.out_f16 = L.out_f16;
+    p.out_fmt = L.out_fmt;
+    p.err = L.err;
     const uint32_t af = L.a_fmt == 1 ? 0u : 1u, bf = L.b_fmt == 1 ? 0u : 1u;   // FMT_E4M3 = 1, FMT_E5M2 = 2
     p.idesc = idesc_f8(pair ? 256 : 128, few ? 128 : 256, af, bf);
     if (few) {
         // Too few 128 x 256 tiles for the SMs: 128 x 128 tiles, K split over a
         // cluster as far as its CTAs all run at once and keep four blocks each.
-        const uint64_t tiles = mt * ((L.N + 127) / 128);
+        const uint64_t tiles = mt * p.side[0].n_tiles;
         uint32_t parts = 1;
         for (uint32_t s = 2; s <= 8; s *= 2) {
             const int fit = L.M <= 32 ? resident_clusters<128, 32>(dev, (int)s) : resident_clusters<128, 128>(dev, (int)s);
-            if (tiles <= (uint64_t)fit && p.kb / s >= 4) parts = s;
+            if (tiles <= (uint64_t)fit && p.side[0].kb / s >= 4) parts = s;
         }
-        p.n_tiles = (L.N + 127) / 128;
         const uint32_t grid = (uint32_t)(tiles * parts);
         e = L.M <= 32 ? launch<128, 32, EPI_STORE, SPLIT>(p, dev, grid, parts, st)
                       : launch<128, 128, EPI_STORE, SPLIT>(p, dev, grid, parts, st);
         if (e != cudaSuccess) { cudaGetLastError(); *why = cudaGetErrorString(e); return 2; }
         return 0;
     }
-    const uint32_t cols = swiglu ? 128 : 256;
-    p.n_tiles = (L.N + cols - 1) / cols;
-    const uint64_t bound = pair ? (L.offsets ? L.M / 256 + L.groups : (L.M + 255) / 256) * (uint64_t)p.n_tiles : mt * p.n_tiles;
+    const uint64_t rows = pair ? 256 : 128;
+    uint64_t bound = (pair ? (L.offsets ? L.M / 256 + L.groups : (L.M + 255) / 256) : mt) * (uint64_t)p.side[0].n_tiles;
+    if (more) bound += (more->M + rows - 1) / rows * p.side[1].n_tiles;
     if (bound >> 31) { *why = "too many tiles"; return 1; }
     const uint64_t fit = pair ? sms / 2 : sms;
     const uint32_t grid = (uint32_t)(bound < fit ? bound : fit) * (pair ? 2 : 1);

@@ -43,6 +43,9 @@ constexpr uint32_t kBoxRows = 32;           // rows of A per TMA box
 constexpr uint32_t kBoxBytes = kBoxRows * kBK;
 constexpr uint32_t kBTile = 128 * kBK;      // 128 rows of B
 
+// Shared memory of the groups' tables.
+__host__ __device__ constexpr uint32_t group_bytes(uint32_t groups) { return 4 * (3 * groups + 1); }
+
 enum Epi { EPI_STORE = 0, EPI_SWIGLU = 1 };
 // SINGLE: one CTA a tile, persistent. PAIR: two CTAs of a cluster share a 256-row tile:
 // tcgen05 cta_group::2 with M = 256, each CTA holding its 128 rows of A and half of B's
@@ -64,26 +67,36 @@ template <int BN, int AR, int MODE> struct Cfg {
     static constexpr uint32_t kOffAmax = kOffOut + 8 * 2048;        // SwiGLU: [2 halves][128] floats
     static constexpr uint32_t kOffBar = kOffAmax + 1024;
     static constexpr uint32_t kOffGroups = kOffBar + 256;           // 3 words per group + 1
-    static constexpr uint32_t kSmem = kOffGroups;                   // + 4 * (3 * groups + 1)
+    static constexpr uint32_t kSmem = kOffGroups;                   // + group_bytes(all_groups)
     static constexpr uint32_t kTmemCols = 2 * BN;
     static_assert(AR * kBK * (kStages - 1) + 128 * kBK <= kOffB + kStages * kBStage, "MMA reads stay inside the ring");
-    static_assert(kSmem + 4 * (3 * kFp8MaxGroups + 1) <= 227 * 1024, "shared memory");
+    static_assert(kSmem + group_bytes(kFp8MaxGroups + 1) <= 227 * 1024, "shared memory");
     static_assert(8 * (2 * kStages + 5) + 8 <= 256, "barriers");
 };
 
-struct Params {
+// One product's operands. A launch walks the tiles of two: the grouped one and, beside
+// it, one more dense product (an expert layer's shared expert, whose few tiles alone
+// would leave most SMs idle).
+struct Side {
     CUtensorMap tm_a;           // A [M][K], box {128, 32}, SW128
     CUtensorMap tm_b0, tm_b1;   // B [groups * N][K], box {128, 128}, SW128 (tm_b1: the up weights, SwiGLU)
     const float *sa;            // [M][kb]
     const float *sb0, *sb1;     // [groups][nb][kb]
-    const int32_t *offsets;     // [groups + 1] or null (one group of M rows)
     void *out;                  // C [M][N], or the 8-bit mid [M][N] of the SwiGLU form
     float *out_scales;          // SwiGLU: [M][nb]
-    uint32_t M, N, K, kb, nb, groups, n_tiles;
+    const float *row_scale;     // factor of each row of C, or null
+    uint32_t M, N, kb, nb, n_tiles;
+    int vec;                    // rows of C start on 16-byte boundaries
+};
+
+struct Params {
+    Side side[2];
+    const int32_t *offsets;     // [groups + 1] or null (one group of all rows)
+    uint32_t groups;            // of side 0; group number `groups` is side 1 where it has rows
+    uint32_t all_groups;        // groups, or groups + 1
     uint32_t idesc;
     int out_f16;
     int out_fmt;                // SwiGLU: 8-bit format of the mid (FMT_*)
-    int vec;                    // rows of C start on 16-byte boundaries
     uint32_t *err;
 };
 
@@ -235,13 +248,13 @@ __device__ __forceinline__ bool promo_any(bool v)
 
 // ---- the tile walk
 struct Groups {
-    const uint32_t *cum;    // [groups + 1] row tiles before group g
-    const uint32_t *row0;   // [groups]
-    const uint32_t *row1;   // [groups]
+    const uint32_t *cum;    // [all_groups + 1] tiles before group g
+    const uint32_t *row0;   // [all_groups]
+    const uint32_t *row1;   // [all_groups]
 };
 
 struct Tile {
-    uint32_t g, m0, m_end, n0;
+    uint32_t g, m0, m_end, n0, side;
 };
 
 // Tile t: groups in order; inside a group the row tile runs fastest, so that the
@@ -249,42 +262,44 @@ struct Tile {
 template <uint32_t ROWS>
 __device__ __forceinline__ Tile tile_at(const Params &p, const Groups &gr, uint32_t t, uint32_t cols)
 {
-    uint32_t lo = 0, hi = p.groups;   // cum[lo] * n_tiles <= t < cum[hi] * n_tiles
+    uint32_t lo = 0, hi = p.all_groups;   // cum[lo] <= t < cum[hi]
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (gr.cum[mid] * p.n_tiles <= t) lo = mid; else hi = mid;
+        if (gr.cum[mid] <= t) lo = mid; else hi = mid;
     }
-    const uint32_t mt = gr.cum[lo + 1] - gr.cum[lo];
-    const uint32_t l = t - gr.cum[lo] * p.n_tiles;
+    const uint32_t mt = (gr.row1[lo] - gr.row0[lo] + ROWS - 1) / ROWS, l = t - gr.cum[lo];
     Tile o;
-    o.g = lo;
+    o.side = lo == p.groups ? 1u : 0u;
+    o.g = o.side ? 0u : lo;
     o.m0 = gr.row0[lo] + (l % mt) * ROWS;
     o.m_end = gr.row1[lo];
     o.n0 = (l / mt) * cols;
     return o;
 }
 
-// Prefix sums of the groups' row tiles (one warp). Offsets are clamped to [0, M]
-// and made ascending, so wrong ones are reported but never lead out of A or C.
+// Prefix sums of the groups' tiles (one warp). Offsets are clamped to [0, M] and made
+// ascending, so wrong ones are reported but never lead out of A or C.
 template <uint32_t ROWS>
 __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uint32_t *row0, uint32_t *row1, uint32_t lane)
 {
-    const uint32_t per = (p.groups + 31) / 32;
+    const uint32_t per = (p.all_groups + 31) / 32;
+    auto tiles = [&](uint32_t g) { return (row1[g] - row0[g] + ROWS - 1) / ROWS * p.side[g == p.groups].n_tiles; };
     uint32_t sum = 0;
     bool bad = false;
     for (uint32_t i = 0; i < per; ++i) {
         const uint32_t g = lane * per + i;
-        if (g >= p.groups) break;
-        uint32_t a = 0, b = p.M;
-        if (p.offsets) {
+        if (g >= p.all_groups) break;
+        uint32_t a = 0, b = p.side[g == p.groups].M;
+        if (p.offsets && g < p.groups) {
             const int32_t o0 = p.offsets[g], o1 = p.offsets[g + 1];
-            a = (uint32_t)min(max((int64_t)o0, (int64_t)0), (int64_t)p.M);
-            b = (uint32_t)min(max((int64_t)o1, (int64_t)a), (int64_t)p.M);
+            const int64_t m = p.side[0].M;
+            a = (uint32_t)min(max((int64_t)o0, (int64_t)0), m);
+            b = (uint32_t)min(max((int64_t)o1, (int64_t)a), m);
             bad |= (int64_t)a != o0 || (int64_t)b != o1;
         }
         row0[g] = a;
         row1[g] = b;
-        sum += (b - a + ROWS - 1) / ROWS;
+        sum += tiles(g);
     }
     if (bad && blockIdx.x == 0) report_error(p.err, kErrBounds, 0xF81);
     uint32_t inc = sum;
@@ -295,11 +310,11 @@ __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uin
     uint32_t base = inc - sum;
     for (uint32_t i = 0; i < per; ++i) {
         const uint32_t g = lane * per + i;
-        if (g >= p.groups) break;
+        if (g >= p.all_groups) break;
         cum[g] = base;
-        base += (row1[g] - row0[g] + ROWS - 1) / ROWS;
+        base += tiles(g);
     }
-    if (lane == 31) cum[p.groups] = inc;
+    if (lane == 31) cum[p.all_groups] = inc;
 }
 
 // ---- epilogue: 32 rows x 64 bytes of a warp through shared memory (2 KB, 16-byte units
@@ -329,13 +344,13 @@ __device__ __forceinline__ void stage_out(const uint8_t *buf, uint32_t lane, uin
 }
 
 // A warp's 32 rows x 64 columns of C from column c: lane = row.
-__device__ __forceinline__ void store_run(const Params &p, const float *acc, uint8_t *buf, uint32_t lane, uint32_t m, uint32_t m_end, uint32_t c)
+__device__ __forceinline__ void store_run(const Side &p, int out_f16, const float *acc, uint8_t *buf, uint32_t lane, uint32_t m, uint32_t m_end, uint32_t c)
 {
-    const uint32_t size = p.out_f16 ? 2u : 4u;
+    const uint32_t size = out_f16 ? 2u : 4u;
     if (p.vec && c + 64 <= p.N) {
         uint8_t *out = static_cast<uint8_t *>(p.out);
         const size_t pitch = (size_t)p.N * size;
-        if (p.out_f16) {
+        if (out_f16) {
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
 #pragma unroll
@@ -374,7 +389,7 @@ __device__ __forceinline__ void store_run(const Params &p, const float *acc, uin
             const float v = *reinterpret_cast<const float *>(buf + r * 64 + (((cc >> 2) ^ (r >> 1)) & 3u) * 16 + (cc & 3) * 4);
             if (m + r < m_end && col < p.N) {
                 const size_t at = (size_t)(m + r) * p.N + col;
-                if (p.out_f16) static_cast<__half *>(p.out)[at] = __float2half_rn(v);
+                if (out_f16) static_cast<__half *>(p.out)[at] = __float2half_rn(v);
                 else static_cast<float *>(p.out)[at] = v;
             }
         }
@@ -406,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *amax_x = reinterpret_cast<float *>(smem + C::kOffAmax);
     uint32_t *cum = reinterpret_cast<uint32_t *>(smem + C::kOffGroups);
-    uint32_t *row0 = cum + p.groups + 1, *row1 = row0 + p.groups;
+    uint32_t *row0 = cum + p.all_groups + 1, *row1 = row0 + p.all_groups;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = MODE == SINGLE ? 0u : cta_rank();
@@ -423,8 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         mbar_init(drain, 1);
         *abort = 0;
         fence_mbar_init();
-        tma_prefetch_desc(&p.tm_a);
-        tma_prefetch_desc(&p.tm_b0);
+        tma_prefetch_desc(&p.side[0].tm_a);
+        tma_prefetch_desc(&p.side[0].tm_b0);
     }
     if (warp == 1) {
         if constexpr (MODE == PAIR) {
@@ -444,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     const Groups gr{cum, row0, row1};
 
     // SPLIT: K blocks [k0, k1) of this CTA. Clusters walk the tiles.
-    uint32_t t0 = blockIdx.x, step = gridDim.x, k0 = 0, k1 = p.kb, parts = 1;
+    uint32_t t0 = blockIdx.x, step = gridDim.x, k0 = 0, parts = 1;
     if constexpr (MODE == PAIR) {
         t0 >>= 1;
         step >>= 1;
@@ -453,10 +468,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(parts));
         t0 = blockIdx.x / parts;
         step = gridDim.x / parts;
-        k0 = (uint32_t)((uint64_t)p.kb * rank / parts);
-        k1 = (uint32_t)((uint64_t)p.kb * (rank + 1) / parts);
+        k0 = (uint32_t)((uint64_t)p.side[0].kb * rank / parts);
     }
-    const uint32_t total = cum[p.groups] * p.n_tiles;
+    const uint32_t total = cum[p.all_groups];
+    // end of a tile's K blocks for this CTA
+    auto k_end = [&](const Side &sd) -> uint32_t {
+        return MODE == SPLIT ? (uint32_t)((uint64_t)sd.kb * (rank + 1) / parts) : sd.kb;
+    };
 
     // BN = 256: a promotion thread keeps 128 accumulators and 64 words in flight, more
     // than the 168 registers it is launched with: 128 * 40 + 256 * 232 = 384 * 168.
@@ -468,15 +486,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         bool alive = true;
         for (uint32_t t = t0; t < total && alive; t += step) {
             const Tile tl = tile_at<C::kTileRows>(p, gr, t, kCols);
+            const Side &sd = p.side[tl.side];
+            const uint32_t k1 = k_end(sd);
             // this CTA's rows of the tile (none for the odd CTA of a short one)
             const uint32_t m0 = tl.m0 + (MODE == PAIR ? rank * kBM : 0u);
             const uint32_t rows = m0 < tl.m_end ? min(tl.m_end - m0, kBM) : 0u, boxes = (rows + kBoxRows - 1) / kBoxRows;
-            const int32_t b_row = (int32_t)(tl.g * p.N + tl.n0);
+            const int32_t b_row = (int32_t)(tl.g * sd.N + tl.n0);
             // the second run: the up weights, or the next 128 columns (none behind the last)
-            const bool two = kRuns == 2 && (E == EPI_SWIGLU || tl.n0 + 128 < p.N);
+            const bool two = kRuns == 2 && (E == EPI_SWIGLU || tl.n0 + 128 < sd.N);
             const bool first = MODE != PAIR || rank == 0, second = two && (MODE != PAIR || rank == 1);
             const uint32_t bytes = boxes * kBoxBytes + (first ? kBTile : 0u) + (second ? kBTile : 0u);
-            const CUtensorMap *tm1 = E == EPI_SWIGLU ? &p.tm_b1 : &p.tm_b0;
+            const CUtensorMap *tma = &sd.tm_a, *tm0 = &sd.tm_b0, *tm1 = E == EPI_SWIGLU ? &sd.tm_b1 : tm0;
             const int32_t b_row1 = b_row + (E == EPI_SWIGLU ? 0 : 128);
             for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
                 const uint32_t st = g % S, ph = (g / S) & 1u;
@@ -487,16 +507,16 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     if constexpr (MODE == PAIR) {
                         const uint32_t bar = peer_addr(&full[st], 0);
                         arrive_expect_tx_cl(bar, bytes);
-                        if (first) tma_load_2d_pair(dB, &p.tm_b0, kc, b_row, bar);
+                        if (first) tma_load_2d_pair(dB, tm0, kc, b_row, bar);
                         if (second) tma_load_2d_pair(dB, tm1, kc, b_row1, bar);
                         for (uint32_t i = 0; i < boxes; ++i)
-                            tma_load_2d_pair(dA + i * kBoxBytes, &p.tm_a, kc, (int32_t)(m0 + i * kBoxRows), bar);
+                            tma_load_2d_pair(dA + i * kBoxBytes, tma, kc, (int32_t)(m0 + i * kBoxRows), bar);
                     } else {
                         mbar_arrive_expect_tx(&full[st], bytes);
-                        tma_load_2d(dB, &p.tm_b0, kc, b_row, &full[st]);
+                        tma_load_2d(dB, tm0, kc, b_row, &full[st]);
                         if (second) tma_load_2d(dB + kBTile, tm1, kc, b_row1, &full[st]);
                         for (uint32_t i = 0; i < boxes; ++i)
-                            tma_load_2d(dA + i * kBoxBytes, &p.tm_a, kc, (int32_t)(m0 + i * kBoxRows), &full[st]);
+                            tma_load_2d(dA + i * kBoxBytes, tma, kc, (int32_t)(m0 + i * kBoxRows), &full[st]);
                     }
                 }
                 __syncwarp();
@@ -513,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         uint32_t g = 0;
         bool alive = true;
         for (uint32_t t = t0; t < total && alive; t += step) {
+            const uint32_t k1 = k_end(p.side[p.all_groups == p.groups ? 0u : tile_at<C::kTileRows>(p, gr, t, kCols).side]);
             for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
                 const uint32_t st = g % S, b = g & 1u;
                 const uint64_t ad = ad0 + st * (C::kAStage >> 4), bd = bd0 + st * (C::kBStage >> 4);
@@ -552,14 +573,16 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         bool alive = true;
         for (uint32_t t = t0; t < total && alive; t += step) {
             const Tile tl = tile_at<C::kTileRows>(p, gr, t, kCols);
+            const Side &sd = p.side[tl.side];
+            const uint32_t k1 = k_end(sd);
             const uint32_t m_warp = tl.m0 + (MODE == PAIR ? rank * kBM : 0u) + quarter * 32, m = m_warp + lane;
             const bool live = m_warp < tl.m_end;   // this warp has rows
             const bool row_ok = m < tl.m_end;
             // run r: accumulator columns [64 half, + 64) of run r's 128
-            const uint32_t nblk = tl.n0 / 128, two = kRuns == 2 && (E == EPI_SWIGLU || nblk + 1 < p.nb) ? 1u : 0u;
-            const float *sa = p.sa + (size_t)(row_ok ? m : tl.m0) * p.kb;
-            const float *sb0 = p.sb0 + ((size_t)tl.g * p.nb + nblk) * p.kb;
-            const float *sb1 = E == EPI_SWIGLU ? p.sb1 + ((size_t)tl.g * p.nb + nblk) * p.kb : sb0 + (size_t)two * p.kb;
+            const uint32_t nblk = tl.n0 / 128, two = kRuns == 2 && (E == EPI_SWIGLU || nblk + 1 < sd.nb) ? 1u : 0u;
+            const float *sa = sd.sa + (size_t)(row_ok ? m : tl.m0) * sd.kb;
+            const float *sb0 = sd.sb0 + ((size_t)tl.g * sd.nb + nblk) * sd.kb;
+            const float *sb1 = E == EPI_SWIGLU ? sd.sb1 + ((size_t)tl.g * sd.nb + nblk) * sd.kb : sb0 + (size_t)two * sd.kb;
             float acc[kRuns * 64];
 #pragma unroll
             for (uint32_t i = 0; i < kRuns * 64; ++i) acc[i] = 0.0f;
@@ -662,13 +685,18 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     }
                     stage_put(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
                 }
-                stage_out(buf, lane, static_cast<uint8_t *>(p.out), p.N, tl.n0 + half * 64, m_warp, tl.m_end);
-                if (row_ok && half == 0) p.out_scales[(size_t)m * p.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
+                stage_out(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
+                if (row_ok && half == 0) sd.out_scales[(size_t)m * sd.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
             } else if (live) {
+                if (sd.row_scale) {
+                    const float f = row_ok ? sd.row_scale[m] : 0.0f;
+#pragma unroll
+                    for (uint32_t i = 0; i < kRuns * 64; ++i) acc[i] *= f;
+                }
 #pragma unroll
                 for (uint32_t r = 0; r < kRuns; ++r) {
                     const uint32_t c = tl.n0 + r * 128 + half * 64;
-                    if (c < p.N) store_run(p, acc + r * 64, buf, lane, m_warp, tl.m_end, c);
+                    if (c < sd.N) store_run(sd, p.out_f16, acc + r * 64, buf, lane, m_warp, tl.m_end, c);
                 }
             }
         }
@@ -691,12 +719,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     if constexpr (MODE == SPLIT) {
         if (t0 < total && !*abort) {
             const Tile tl = tile_at<C::kTileRows>(p, gr, t0, kCols);
+            const Side &sd = p.side[0];
             const uint32_t rows = min(tl.m_end - tl.m0, kBM), base = smem_u32(smem);
             // the cluster's CTAs take every parts-th 16-byte column of the tile, summed in rank order
             for (uint32_t i = threadIdx.x * parts + rank; i < rows * (BN / 4); i += kThreads * parts) {
                 const uint32_t r = i / (BN / 4), c4 = i % (BN / 4);
                 const uint32_t c = tl.n0 + 4 * c4;
-                if (c >= p.N) continue;
+                if (c >= sd.N) continue;
                 const uint32_t at = base + 16 * (r * (BN / 4) + ((c4 + r) & (BN / 4 - 1)));
                 float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (uint32_t q = 0; q < parts; ++q) {
@@ -707,26 +736,26 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer));
                     s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
                 }
-                const size_t o = (size_t)(tl.m0 + r) * p.N + c;
+                const size_t o = (size_t)(tl.m0 + r) * sd.N + c;
                 if (p.out_f16) {
-                    __half *d = static_cast<__half *>(p.out) + o;
-                    if (p.vec && c + 4 <= p.N) {
+                    __half *d = static_cast<__half *>(sd.out) + o;
+                    if (sd.vec && c + 4 <= sd.N) {
                         *reinterpret_cast<uint2 *>(d) = make_uint2(half2_bits(s.x, s.y), half2_bits(s.z, s.w));
                     } else {
                         d[0] = __float2half_rn(s.x);
-                        if (c + 1 < p.N) d[1] = __float2half_rn(s.y);
-                        if (c + 2 < p.N) d[2] = __float2half_rn(s.z);
-                        if (c + 3 < p.N) d[3] = __float2half_rn(s.w);
+                        if (c + 1 < sd.N) d[1] = __float2half_rn(s.y);
+                        if (c + 2 < sd.N) d[2] = __float2half_rn(s.z);
+                        if (c + 3 < sd.N) d[3] = __float2half_rn(s.w);
                     }
                 } else {
-                    float *d = static_cast<float *>(p.out) + o;
-                    if (p.vec && c + 4 <= p.N) {
+                    float *d = static_cast<float *>(sd.out) + o;
+                    if (sd.vec && c + 4 <= sd.N) {
                         *reinterpret_cast<float4 *>(d) = s;
                     } else {
                         d[0] = s.x;
-                        if (c + 1 < p.N) d[1] = s.y;
-                        if (c + 2 < p.N) d[2] = s.z;
-                        if (c + 3 < p.N) d[3] = s.w;
+                        if (c + 1 < sd.N) d[1] = s.y;
+                        if (c + 2 < sd.N) d[2] = s.z;
+                        if (c + 3 < sd.N) d[3] = s.w;
                     }
                 }
             }

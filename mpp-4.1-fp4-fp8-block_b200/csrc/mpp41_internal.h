@@ -125,6 +125,8 @@ struct Fp8Launch {
     uint32_t M, N, K, groups;
     int a_fmt, b_fmt, out_fmt;   // FMT_E4M3 (1) or FMT_E5M2 (2)
     int out_f16;
+    const float *row_scale;      // factor of each row of the result, or null
+    const Fp8Launch *more;       // one more dense product in the same launch (same formats and output type), or null
     uint32_t *err;
 };
 int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why);
@@ -137,12 +139,12 @@ cudaError_t launch_quantize_weights_fp8(int fmt, const float *w, uint32_t N, uin
 
 // Pieces of the FP8 expert layer (mpp41_moe_fp8.cu): n = T * k assignments; H % 128 == 0,
 // x 32-byte aligned; xq / xs (the unscattered rows) may be null.
-cudaError_t launch_fp8_plan(const int32_t *ids, uint32_t n, uint32_t E, int32_t *offsets, int32_t *inv, uint32_t *err,
-                            cudaStream_t st);
+cudaError_t launch_fp8_plan(const int32_t *ids, const float *weights, uint32_t n, uint32_t E, int32_t *offsets,
+                            int32_t *inv, float *row_weight, uint32_t *err, cudaStream_t st);
 cudaError_t launch_fp8_scatter(int fmt, const void *x, uint32_t T, uint32_t H, const int32_t *inv, uint32_t k, uint8_t *pq,
                                float *ps, uint8_t *xq, float *xs, cudaStream_t st);
-cudaError_t launch_fp8_combine(const float *y, const int32_t *inv, const float *w, uint32_t T, uint32_t k, uint32_t H,
-                               const float *shared_y, void *out, int out_f16, cudaStream_t st);
+cudaError_t launch_fp8_combine(const void *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const void *shared_y,
+                               void *out, int f16, cudaStream_t st);
 
 // Expert routing with scores, balance bias and groups (mpp41_moe_gate.cu): E <= 512,
 // k <= 32, groups <= 32 dividing E.

@@ -6,8 +6,12 @@
 //   scatter:  x is quantized once (1 x 128 scales) and each block written to the
 //             rows of its token's assignments; no gather pass reads it again.
 //   experts:  grouped gate/up product with the SwiGLU + quantization epilogue, then
-//             the grouped down product -> y [rows][H] fp32.
-//   combine:  out[t] = shared(t) + sum_j weights[t][j] * y[inv[t*k+j]], in slot order.
+//             the grouped down product, each row times its routing weight
+//             -> y [rows][H]; the shared expert's tiles run in the same two launches.
+//   combine:  out[t] = shared(t) + sum_j y[inv[t*k+j]], in slot order, summed in fp32.
+// y has out's type. For fp16 out the weighted rows are rounded to fp16 (2^-11 of each
+// term, as the sum's own rounding; terms beyond 65504 need a sum that is too): half the
+// bytes between the products and the combine, which at 2000 tokens are 0.9 GB in fp32.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -25,9 +29,9 @@ constexpr int kPlanThreads = 512;
 // One CTA an expert, each reading all ids twice (they sit in L2): rows before this
 // expert's = ids below it, then a stable compaction. Threads own contiguous runs
 // of assignments, so one block scan orders them. No launch or wait joins the CTAs.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__restrict__ ids, uint32_t n, uint32_t E,
-                                                            int32_t *__restrict__ offsets, int32_t *__restrict__ inv,
-                                                            uint32_t *err)
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__restrict__ ids, const float *__restrict__ weights,
+                                                            uint32_t n, uint32_t E, int32_t *__restrict__ offsets,
+                                                            int32_t *__restrict__ inv, float *__restrict__ row_weight, uint32_t *err)
 {
     __shared__ uint32_t sh_lt[kPlanThreads / 32], sh_eq[kPlanThreads / 32];
     const int32_t e = (int32_t)blockIdx.x;
@@ -71,7 +75,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__res
     uint32_t row = base + before + inc - eq;
     if (eq)
         for (uint32_t a = a0; a < a1; ++a)
-            if (ids[a] == e) inv[a] = (int32_t)row++;
+            if (ids[a] == e) {
+                row_weight[row] = weights[a];
+                inv[a] = (int32_t)row++;
+            }
 }
 
 // As the activation quantizer (8 lanes a block of 128, 16 values a lane), each block
@@ -109,37 +116,51 @@ __global__ void __launch_bounds__(256) quant_scatter_kernel(const uint8_t *__res
     }
 }
 
-// One CTA per (token, 1024 columns); slots summed in order, fp32.
-__global__ void __launch_bounds__(256) combine_fp8_kernel(const float *__restrict__ y, const int32_t *__restrict__ inv,
-                                                          const float *__restrict__ w, uint32_t k, uint32_t H,
-                                                          const float *__restrict__ shared_y, void *__restrict__ out, int out_f16)
+// One CTA per (token, 2048 or 1024 columns): 16 bytes a thread; slots summed in order, fp32.
+template <bool F16>
+__global__ void __launch_bounds__(256) combine_fp8_kernel(const uint4 *__restrict__ y, const int32_t *__restrict__ inv,
+                                                          uint32_t k, uint32_t row16, const uint4 *__restrict__ shared_y,
+                                                          uint4 *__restrict__ out)
 {
+    constexpr int V = F16 ? 8 : 4;
     const uint32_t t = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
-    if (c >= H / 4) return;
-    float4 acc = shared_y ? __ldcs(reinterpret_cast<const float4 *>(shared_y + (size_t)t * H) + c) : make_float4(0, 0, 0, 0);
+    if (c >= row16) return;
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+    auto add = [&](const uint4 &v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (F16) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                acc[(2 * i) % V] += f.x;
+                acc[(2 * i + 1) % V] += f.y;
+            } else {
+                acc[i] += __uint_as_float(w[i]);
+            }
+        }
+    };
+    if (shared_y) add(__ldcs(shared_y + (size_t)t * row16 + c));
 #pragma unroll 4
     for (uint32_t j = 0; j < k; ++j) {
         const int32_t r = inv[(size_t)t * k + j];
-        if (r < 0) continue;
-        const float wt = w[(size_t)t * k + j];
-        const float4 v = __ldcs(reinterpret_cast<const float4 *>(y + (size_t)r * H) + c);
-        acc.x = fmaf(wt, v.x, acc.x);
-        acc.y = fmaf(wt, v.y, acc.y);
-        acc.z = fmaf(wt, v.z, acc.z);
-        acc.w = fmaf(wt, v.w, acc.w);
+        if (r >= 0) add(__ldcs(y + (size_t)r * row16 + c));
     }
-    if (out_f16)
-        reinterpret_cast<uint2 *>(static_cast<__half *>(out) + (size_t)t * H)[c] = make_uint2(half2_bits(acc.x, acc.y), half2_bits(acc.z, acc.w));
+    uint4 o;
+    if (F16)
+        o = make_uint4(half2_bits(acc[0], acc[1]), half2_bits(acc[2], acc[3]), half2_bits(acc[4 % V], acc[5 % V]), half2_bits(acc[6 % V], acc[7 % V]));
     else
-        reinterpret_cast<float4 *>(static_cast<float *>(out) + (size_t)t * H)[c] = acc;
+        o = make_uint4(__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3]));
+    out[(size_t)t * row16 + c] = o;
 }
 
 }  // namespace fp8
 
-cudaError_t launch_fp8_plan(const int32_t *ids, uint32_t n, uint32_t E, int32_t *offsets, int32_t *inv, uint32_t *err,
-                            cudaStream_t st)
+cudaError_t launch_fp8_plan(const int32_t *ids, const float *weights, uint32_t n, uint32_t E, int32_t *offsets,
+                            int32_t *inv, float *row_weight, uint32_t *err, cudaStream_t st)
 {
-    fp8::plan_kernel<<<E, fp8::kPlanThreads, 0, st>>>(ids, n, E, offsets, inv, err);
+    fp8::plan_kernel<<<E, fp8::kPlanThreads, 0, st>>>(ids, weights, n, E, offsets, inv, row_weight, err);
     return cudaGetLastError();
 }
 
@@ -154,11 +175,14 @@ cudaError_t launch_fp8_scatter(int fmt, const void *x, uint32_t T, uint32_t H, c
     return cudaGetLastError();
 }
 
-cudaError_t launch_fp8_combine(const float *y, const int32_t *inv, const float *w, uint32_t T, uint32_t k, uint32_t H,
-                               const float *shared_y, void *out, int out_f16, cudaStream_t st)
+cudaError_t launch_fp8_combine(const void *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const void *shared_y,
+                               void *out, int f16, cudaStream_t st)
 {
-    const dim3 grid(T, (H / 4 + 255) / 256);
-    fp8::combine_fp8_kernel<<<grid, 256, 0, st>>>(y, inv, w, k, H, shared_y, out, out_f16);
+    const uint32_t row16 = H / (f16 ? 8 : 4);
+    const dim3 grid(T, (row16 + 255) / 256);
+    const uint4 *a = static_cast<const uint4 *>(y), *s = static_cast<const uint4 *>(shared_y);
+    if (f16) fp8::combine_fp8_kernel<true><<<grid, 256, 0, st>>>(a, inv, k, row16, s, static_cast<uint4 *>(out));
+    else fp8::combine_fp8_kernel<false><<<grid, 256, 0, st>>>(a, inv, k, row16, s, static_cast<uint4 *>(out));
     return cudaGetLastError();
 }
 
