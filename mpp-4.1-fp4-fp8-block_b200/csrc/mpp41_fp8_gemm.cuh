@@ -17,8 +17,8 @@
 // pair instead of a shared-memory read per column. Row blocks past the tile's end
 // are neither loaded nor promoted (32-row granularity).
 //
-// Warp roles (384 threads): 0 TMA producer, 1 MMA issuer and TMEM owner, 2..3 idle (they
-// hold registers that the promotion warps take over), 4..11 promotion (warp w: TMEM lane
+// Warp roles (384 threads): 0 TMA producer of B, 1 MMA issuer and TMEM owner, 2 TMA
+// producer of A, 3 idle (it holds registers that the promotion warps take over), 4..11 promotion (warp w: TMEM lane
 // quarter w % 4, column half (w - 4) / 4). One warp for copies and MMAs ran the
 // 4096 x 14336 x 4096 product a third slower: a block's copies take it as long to issue
 // as the block's MMAs take to run.
@@ -39,8 +39,6 @@ constexpr uint32_t kBM = 128;
 constexpr uint32_t kBK = 128;               // one scale block, one 128-byte swizzle atom
 constexpr int kThreads = 384;
 constexpr int kPromoThreads = 256;
-constexpr uint32_t kBoxRows = 32;           // rows of A per TMA box
-constexpr uint32_t kBoxBytes = kBoxRows * kBK;
 constexpr uint32_t kBTile = 128 * kBK;      // 128 rows of B
 
 // Shared memory of the groups' tables.
@@ -68,17 +66,17 @@ template <int BN, int AR, int MODE> struct Cfg {
     static constexpr uint32_t kOffBar = kOffAmax + 1024;
     static constexpr uint32_t kOffGroups = kOffBar + 256;           // 3 words per group + 1
     static constexpr uint32_t kSmem = kOffGroups;                   // + group_bytes(all_groups)
-    static constexpr uint32_t kTmemCols = 2 * BN;
+    static constexpr uint32_t kAccs = 512 / BN;                     // accumulators in tensor memory, all of it
     static_assert(AR * kBK * (kStages - 1) + 128 * kBK <= kOffB + kStages * kBStage, "MMA reads stay inside the ring");
     static_assert(kSmem + group_bytes(kFp8MaxGroups + 1) <= 227 * 1024, "shared memory");
-    static_assert(8 * (2 * kStages + 5) + 8 <= 256, "barriers");
+    static_assert(8 * (2 * kStages + 2 * kAccs + 1) + 8 <= 256, "barriers");
 };
 
 // One product's operands. A launch walks the tiles of two: the grouped one and, beside
 // it, one more dense product (an expert layer's shared expert, whose few tiles alone
 // would leave most SMs idle).
 struct Side {
-    CUtensorMap tm_a;           // A [M][K], box {128, 32}, SW128
+    CUtensorMap tm_a;           // A [M][K], box {128, box_rows}, SW128
     CUtensorMap tm_b0, tm_b1;   // B [groups * N][K], box {128, 128}, SW128 (tm_b1: the up weights, SwiGLU)
     const float *sa;            // [M][kb]
     const float *sb0, *sb1;     // [groups][nb][kb]
@@ -95,43 +93,40 @@ struct Params {
     uint32_t groups;            // of side 0; group number `groups` is side 1 where it has rows
     uint32_t all_groups;        // groups, or groups + 1
     uint32_t idesc;
+    uint32_t box_rows;          // rows of A a copy brings (32 or 128)
     int out_f16;
     int out_fmt;                // SwiGLU: 8-bit format of the mid (FMT_*)
     uint32_t *err;
 };
 
-// Bounded wait for the handshakes between the MMA issuer and the promotion warps. The
-// bound is a number of tries, each suspended for at most kTryNs by the hardware: about
-// kWaitLimitNs in all, and no timer to keep in the promotion warps' last registers.
-constexpr uint32_t kTryNs = 4096, kTries = (uint32_t)(kWaitLimitNs / kTryNs);
-
-__device__ __forceinline__ bool try_wait_ns(uint32_t addr, uint32_t parity)
+// Bounded wait of a converged warp for an mbarrier phase, with one outcome for the warp.
+// The roles hand over to one another every K block, so the usual case is one poll that
+// succeeds (13 cycles) and a vote (17); a try_wait with a time limit of its own takes 59,
+// the limit's timer is read every 64th poll only. Two such waits at 94 cycles each paced
+// the MMA issuer.
+__device__ __forceinline__ bool wait_slow(uint32_t addr, uint32_t parity, volatile int *abort, uint32_t *err, uint32_t site)
 {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(addr), "r"(parity), "n"(kTryNs) : "memory");
-    return ok != 0;
-}
-
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err, uint32_t site)
-{
-    const uint32_t addr = smem_u32(bar);
-    for (uint32_t it = 0; it < kTries; ++it) {
-        if (try_wait_ns(addr, parity)) return true;
-        if (*abort) return false;
+    uint64_t t0 = 0;
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(addr, parity)) return true;
+        if ((it & 63u) == 0) {
+            if (*abort) return false;
+            const uint64_t now = globaltimer_ns();
+            if (!t0) t0 = now;
+            if (now - t0 > kWaitLimitNs) {
+                report_error(err, kErrTimeout, site);
+                *abort = 1;
+                return false;
+            }
+        }
     }
-    report_error(err, kErrTimeout, site);
-    *abort = 1;
-    return false;
 }
 
-// By all lanes of a converged warp, with one outcome.
 __device__ __forceinline__ bool wait_all(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err, uint32_t site)
 {
-    return __all_sync(0xffffffffu, wait(bar, parity, abort, err, site));
+    const uint32_t addr = smem_u32(bar);
+    if (__all_sync(0xffffffffu, mbar_try_wait(addr, parity))) return true;
+    return __all_sync(0xffffffffu, wait_slow(addr, parity, abort, err, site));
 }
 
 // Instruction descriptor, kind::f8f6f4, fp32 D, both operands K-major; formats 0 = E4M3, 1 = E5M2.
@@ -404,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 {
     using C = Cfg<BN, AR, MODE>;
     constexpr int S = C::kStages;
+    constexpr uint32_t NA = C::kAccs;
     constexpr uint32_t kRuns = C::kRuns;     // a promotion thread has 64 columns of each run
     constexpr uint32_t kCols = E == EPI_SWIGLU ? BN / 2 : BN;   // output columns per tile
     // The kernel has no static shared memory, so the dynamic part starts on its alignment.
@@ -416,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     }
     uint8_t *sA = smem, *sB = smem + C::kOffB;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kOffBar);
-    uint64_t *full = bars, *empty = bars + S, *acc_full = empty + S, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
+    uint64_t *full = bars, *empty = bars + S, *acc_full = empty + S, *acc_empty = acc_full + NA, *drain = acc_empty + NA;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *amax_x = reinterpret_cast<float *>(smem + C::kOffAmax);
@@ -428,10 +424,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     if (threadIdx.x == 0) {
         constexpr uint32_t kSides = MODE == PAIR ? 2 : 1;   // the even CTA's full / acc_empty count both CTAs
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full[s], kSides);
+            mbar_init(&full[s], 2 * kSides);
             mbar_init(&empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (uint32_t b = 0; b < NA; ++b) {
             mbar_init(&acc_full[b], 1);
             mbar_init(&acc_empty[b], 8 * kSides);
         }
@@ -443,14 +439,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     }
     if (warp == 1) {
         if constexpr (MODE == PAIR) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemCols) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         } else {
-            tmem_alloc(tmem_slot, C::kTmemCols);
+            tmem_alloc(tmem_slot, 512);
             tmem_relinquish();
         }
     }
-    if (warp == 2) build_groups<C::kTileRows>(p, cum, row0, row1, lane);
+    if (warp == 3) build_groups<C::kTileRows>(p, cum, row0, row1, lane);
     tc_fence_before();
     __syncthreads();
     if constexpr (MODE == PAIR) cluster_sync();   // the peer's barriers are initialised before any remote arrive
@@ -480,46 +476,49 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     // than the 168 registers it is launched with: 128 * 40 + 256 * 232 = 384 * 168.
     if (warp < 4) {
       if constexpr (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-      if (warp == 0) {
-        // ------------------------------------------------ TMA producer
-        uint32_t g = 0;
+      if (warp == 0 || warp == 2) {
+        // ------------------------------------------------ TMA producers: 0 B, 2 A
+        // (one warp issuing a stage's copies one after the other paces small tiles)
+        const bool is_b = warp == 0;
+        uint8_t *ring = is_b ? sB : sA;
+        const uint32_t stage = is_b ? C::kBStage : C::kAStage;
+        uint32_t st = 0, ph = 1, g = 0;
         bool alive = true;
         for (uint32_t t = t0; t < total && alive; t += step) {
             const Tile tl = tile_at<C::kTileRows>(p, gr, t, kCols);
             const Side &sd = p.side[tl.side];
             const uint32_t k1 = k_end(sd);
-            // this CTA's rows of the tile (none for the odd CTA of a short one)
-            const uint32_t m0 = tl.m0 + (MODE == PAIR ? rank * kBM : 0u);
-            const uint32_t rows = m0 < tl.m_end ? min(tl.m_end - m0, kBM) : 0u, boxes = (rows + kBoxRows - 1) / kBoxRows;
-            const int32_t b_row = (int32_t)(tl.g * sd.N + tl.n0);
-            // the second run: the up weights, or the next 128 columns (none behind the last)
+            // copies of this CTA for a block: row i * rows_per of its first, and how many.
+            // A: its rows of the tile (none for the odd CTA of a short one). B: a copy a run;
+            // the second run is the up weights, or the next 128 columns (none behind the last).
+            const uint32_t m0 = tl.m0 + (MODE == PAIR ? rank * kBM : 0u), rows = m0 < tl.m_end ? min(tl.m_end - m0, kBM) : 0u;
             const bool two = kRuns == 2 && (E == EPI_SWIGLU || tl.n0 + 128 < sd.N);
             const bool first = MODE != PAIR || rank == 0, second = two && (MODE != PAIR || rank == 1);
-            const uint32_t bytes = boxes * kBoxBytes + (first ? kBTile : 0u) + (second ? kBTile : 0u);
-            const CUtensorMap *tma = &sd.tm_a, *tm0 = &sd.tm_b0, *tm1 = E == EPI_SWIGLU ? &sd.tm_b1 : tm0;
-            const int32_t b_row1 = b_row + (E == EPI_SWIGLU ? 0 : 128);
+            const uint32_t box = is_b ? 128u : p.box_rows;
+            const uint32_t copies = is_b ? (first ? 1u : 0u) + (second ? 1u : 0u) : (rows + box - 1) / box;
+            const CUtensorMap *tm = is_b ? (first || E != EPI_SWIGLU ? &sd.tm_b0 : &sd.tm_b1) : &sd.tm_a;
+            const CUtensorMap *tm1 = is_b && E == EPI_SWIGLU ? &sd.tm_b1 : tm;
+            const int32_t row = is_b ? (int32_t)(tl.g * sd.N + tl.n0) + (first || E == EPI_SWIGLU ? 0 : 128) : (int32_t)m0;
+            const int32_t row_step = is_b && E == EPI_SWIGLU ? 0 : (int32_t)box;
+            const uint32_t box_bytes = box * kBK, bytes = copies * box_bytes;
             for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
-                const uint32_t st = g % S, ph = (g / S) & 1u;
-                if (!wait_all(&empty[st], ph ^ 1u, abort, p.err, 0xF01)) { alive = false; break; }
+                if (!wait_all(&empty[st], ph, abort, p.err, 0xF01)) { alive = false; break; }
                 if (elect_one_sync()) {
                     const int32_t kc = (int32_t)(kk * kBK);
-                    uint8_t *dA = sA + st * C::kAStage, *dB = sB + st * C::kBStage;
+                    uint8_t *dst = ring + st * stage;
                     if constexpr (MODE == PAIR) {
                         const uint32_t bar = peer_addr(&full[st], 0);
                         arrive_expect_tx_cl(bar, bytes);
-                        if (first) tma_load_2d_pair(dB, tm0, kc, b_row, bar);
-                        if (second) tma_load_2d_pair(dB, tm1, kc, b_row1, bar);
-                        for (uint32_t i = 0; i < boxes; ++i)
-                            tma_load_2d_pair(dA + i * kBoxBytes, tma, kc, (int32_t)(m0 + i * kBoxRows), bar);
+                        for (uint32_t i = 0; i < copies; ++i)
+                            tma_load_2d_pair(dst + i * box_bytes, i ? tm1 : tm, kc, row + (int32_t)i * row_step, bar);
                     } else {
                         mbar_arrive_expect_tx(&full[st], bytes);
-                        tma_load_2d(dB, tm0, kc, b_row, &full[st]);
-                        if (second) tma_load_2d(dB + kBTile, tm1, kc, b_row1, &full[st]);
-                        for (uint32_t i = 0; i < boxes; ++i)
-                            tma_load_2d(dA + i * kBoxBytes, tma, kc, (int32_t)(m0 + i * kBoxRows), &full[st]);
+                        for (uint32_t i = 0; i < copies; ++i)
+                            tma_load_2d(dst + i * box_bytes, i ? tm1 : tm, kc, row + (int32_t)i * row_step, &full[st]);
                     }
                 }
                 __syncwarp();
+                if (++st == (uint32_t)S) { st = 0; ph ^= 1u; }
             }
         }
         // drain: no copy may still be landing when the CTA exits (PAIR: the even CTA's
@@ -530,15 +529,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
       } else if (warp == 1 && (MODE != PAIR || rank == 0)) {
         // ------------------------------------------------ MMA issuer
         const uint64_t ad0 = smem_desc_sw128(sA), bd0 = smem_desc_sw128(sB);
-        uint32_t g = 0;
+        uint32_t st = 0, ph = 0, b = 0, bph = 1;
         bool alive = true;
         for (uint32_t t = t0; t < total && alive; t += step) {
             const uint32_t k1 = k_end(p.side[p.all_groups == p.groups ? 0u : tile_at<C::kTileRows>(p, gr, t, kCols).side]);
-            for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
-                const uint32_t st = g % S, b = g & 1u;
+            for (uint32_t kk = k0; kk < k1; ++kk) {
                 const uint64_t ad = ad0 + st * (C::kAStage >> 4), bd = bd0 + st * (C::kBStage >> 4);
-                if (!wait_all(&full[st], (g / S) & 1u, abort, p.err, 0xF04) ||
-                    !wait_all(&acc_empty[b], ((g >> 1) & 1u) ^ 1u, abort, p.err, 0xF03)) { alive = false; break; }
+                if (!wait_all(&full[st], ph, abort, p.err, 0xF04) ||
+                    !wait_all(&acc_empty[b], bph, abort, p.err, 0xF03)) { alive = false; break; }
                 tc_fence_after();
                 if (elect_one_sync()) {
 #pragma unroll
@@ -555,6 +553,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     }
                 }
                 __syncwarp();
+                if (++st == (uint32_t)S) { st = 0; ph ^= 1u; }
+                if (++b == NA) { b = 0; bph ^= 1u; }
             }
         }
         if (elect_one_sync()) {
@@ -612,8 +612,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     for (uint32_t i = 0; i < 2; ++i) {
                         if (kq + i >= k1) break;
                         fetch(kq + i + 1, i ^ 1u);
-                        const uint32_t b = g & 1u;
-                        if (!wait_all(&acc_full[b], (g >> 1) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
+                        const uint32_t b = g % NA;
+                        if (!wait_all(&acc_full[b], (g / NA) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
                         ++g;
                         tc_fence_after();
                         const uint32_t base = tmem + lane_base + b * BN + half * 64;
@@ -638,8 +638,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 }
             } else {
                 for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
-                    if (!wait_all(&acc_full[g & 1u], (g >> 1) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
-                    release(g & 1u);
+                    if (!wait_all(&acc_full[g % NA], (g / NA) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
+                    release(g % NA);
                 }
             }
             if (E != EPI_SWIGLU && !alive) break;
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     const uint32_t r = quarter * 32 + lane;
 #pragma unroll
                     for (uint32_t i = 0; i < kRuns * 16; ++i) {
-                        const uint32_t c4 = half * 16 + i;
+                        const uint32_t c4 = i / 16 * 32 + half * 16 + i % 16;
                         part[r * (BN / 4) + ((c4 + r) & (BN / 4 - 1))] =
                             make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
                     }
@@ -713,8 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     if (warp == 1) {
         tc_fence_after();
         if constexpr (MODE == PAIR)
-            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmemCols) : "memory");
-        else tmem_dealloc(tmem, C::kTmemCols);
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        else tmem_dealloc(tmem, 512);
     }
     if constexpr (MODE == SPLIT) {
         if (t0 < total && !*abort) {
