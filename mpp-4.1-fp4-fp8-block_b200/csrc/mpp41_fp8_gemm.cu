@@ -70,16 +70,18 @@ cudaError_t launch(const Params &p, int dev, uint32_t grid, uint32_t parts, cuda
     cudaError_t e = prepare<BN, AR, E, MODE>(dev);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = parts;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = parts;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Cfg<BN, AR, MODE>::kSmem + group_bytes(p.all_groups);
     cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = MODE == SINGLE ? 0 : 1;
+    cfg.attrs = at;
+    cfg.numAttrs = MODE == SINGLE ? 0 : MODE == PAIR ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<BN, AR, E, MODE>, p);
 }
 

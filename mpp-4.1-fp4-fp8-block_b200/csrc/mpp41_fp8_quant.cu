@@ -23,6 +23,8 @@ template <int FMT>
 __global__ void __launch_bounds__(256) quant_act_kernel(const uint8_t *__restrict__ x, uint32_t H, uint32_t kb,
                                                         uint64_t blocks, uint8_t *__restrict__ q, float *__restrict__ scales)
 {
+    pdl_launch_dependents();
+    pdl_wait_prior();
     const uint32_t sub = threadIdx.x & 7;
     const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 8);
     for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 8) + threadIdx.x / 8; __any_sync(0xffffffffu, i < blocks); i += step) {
@@ -46,6 +48,8 @@ template <int FMT>
 __global__ void __launch_bounds__(256) quant_act_any_kernel(const __half *__restrict__ x, uint32_t H, uint32_t kb,
                                                             uint64_t blocks, uint8_t *__restrict__ q, float *__restrict__ scales)
 {
+    pdl_launch_dependents();
+    pdl_wait_prior();
     const uint32_t lane = threadIdx.x & 31;
     const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 32);
     for (uint64_t i = (uint64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32; i < blocks; i += step) {
@@ -78,6 +82,8 @@ __global__ void __launch_bounds__(256) quant_weights_kernel(const float *__restr
                                                             uint8_t *__restrict__ q, float *__restrict__ scales)
 {
     __shared__ float part[8];
+    pdl_launch_dependents();
+    pdl_wait_prior();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t bn = blockIdx.x / kb, bk = blockIdx.x - bn * kb;
     const uint32_t c = bk * kBlock + 4 * lane;
@@ -142,11 +148,9 @@ cudaError_t launch_quantize_act_fp8(int fmt, const void *x, uint32_t T, uint32_t
     const unsigned grid = (unsigned)(need < 148 * 16 ? need : 148 * 16);
     const uint8_t *xb = static_cast<const uint8_t *>(x);
     const __half *xh = static_cast<const __half *>(x);
-    if (wide && fmt == 1) quant_act_kernel<1><<<grid, 256, 0, st>>>(xb, H, kb, blocks, q, scales);
-    else if (wide) quant_act_kernel<2><<<grid, 256, 0, st>>>(xb, H, kb, blocks, q, scales);
-    else if (fmt == 1) quant_act_any_kernel<1><<<grid, 256, 0, st>>>(xh, H, kb, blocks, q, scales);
-    else quant_act_any_kernel<2><<<grid, 256, 0, st>>>(xh, H, kb, blocks, q, scales);
-    return cudaGetLastError();
+    if (wide)
+        return launch_overlapped(fmt == 1 ? quant_act_kernel<1> : quant_act_kernel<2>, dim3(grid), dim3(256), 0, st, xb, H, kb, blocks, q, scales);
+    return launch_overlapped(fmt == 1 ? quant_act_any_kernel<1> : quant_act_any_kernel<2>, dim3(grid), dim3(256), 0, st, xh, H, kb, blocks, q, scales);
 }
 
 cudaError_t launch_quantize_weights_fp8(int fmt, const float *w, uint32_t N, uint32_t K, uint8_t *q, float *scales, cudaStream_t st)
@@ -156,11 +160,9 @@ cudaError_t launch_quantize_weights_fp8(int fmt, const float *w, uint32_t N, uin
     const uint32_t kb = (K + kBlock - 1) / kBlock, nb = (N + kBlock - 1) / kBlock;
     const bool vec = K % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && (reinterpret_cast<uintptr_t>(q) & 3u) == 0;
     const unsigned grid = nb * kb;   // the caller keeps it below 2^31
-    if (vec && fmt == 1) quant_weights_kernel<1, true><<<grid, 256, 0, st>>>(w, N, K, kb, q, scales);
-    else if (vec) quant_weights_kernel<2, true><<<grid, 256, 0, st>>>(w, N, K, kb, q, scales);
-    else if (fmt == 1) quant_weights_kernel<1, false><<<grid, 256, 0, st>>>(w, N, K, kb, q, scales);
-    else quant_weights_kernel<2, false><<<grid, 256, 0, st>>>(w, N, K, kb, q, scales);
-    return cudaGetLastError();
+    return launch_overlapped(vec ? (fmt == 1 ? quant_weights_kernel<1, true> : quant_weights_kernel<2, true>)
+                                 : (fmt == 1 ? quant_weights_kernel<1, false> : quant_weights_kernel<2, false>),
+                             dim3(grid), dim3(256), 0, st, w, N, K, kb, q, scales);
 }
 
 }  // namespace mpp41

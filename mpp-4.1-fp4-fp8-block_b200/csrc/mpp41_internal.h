@@ -109,6 +109,24 @@ struct MxLaunch {
 };
 int launch_mxf4_gemm(const MxLaunch &L, cudaStream_t st, const char **why);
 
+// Launch whose start overlaps the end of the kernel before it on the stream; the kernel
+// calls pdl_wait_prior() before it touches global memory.
+template <typename... K, typename... A>
+cudaError_t launch_overlapped(void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
+{
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+}
+
 // FP8 products with fp32 scales per block of 128 (mpp41_fp8_gemm.cuh): A [M][K]
 // with scales [M][K/128], B [groups * N][K] with scales [groups][N/128][K/128];
 // rows [offsets[g], offsets[g+1]) meet B[g] (offsets null: one group). With b1

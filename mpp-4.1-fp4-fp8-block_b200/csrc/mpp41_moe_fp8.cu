@@ -180,9 +180,9 @@ cudaError_t launch_fp8_combine(const void *y, const int32_t *inv, uint32_t T, ui
 {
     const uint32_t row16 = H / (f16 ? 8 : 4);
     const dim3 grid(T, (row16 + 255) / 256);
-    const uint4 *a = static_cast<const uint4 *>(y), *s = static_cast<const uint4 *>(shared_y);
-    if (f16) fp8::combine_fp8_kernel<true><<<grid, 256, 0, st>>>(a, inv, k, row16, s, static_cast<uint4 *>(out));
-    else fp8::combine_fp8_kernel<false><<<grid, 256, 0, st>>>(a, inv, k, row16, s, static_cast<uint4 *>(out));
+    const uint4 *a = static_cast<const uint4 *>(y), *sy = static_cast<const uint4 *>(shared_y);
+    if (f16) fp8::combine_fp8_kernel<true><<<grid, 256, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
+    else fp8::combine_fp8_kernel<false><<<grid, 256, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
     return cudaGetLastError();
 }
 

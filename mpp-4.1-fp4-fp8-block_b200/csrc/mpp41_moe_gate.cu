@@ -258,6 +258,8 @@ __global__ void __launch_bounds__(32 * kWarps) any_kernel(const Params p)
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double *sv = smem + (size_t)warp * p.E;
     const uint32_t t = blockIdx.x * kWarps + warp;
+    pdl_launch_dependents();
+    pdl_wait_prior();
     if (t >= p.T) return;
     const size_t row = (size_t)t * p.E;
     float z[PER];
@@ -347,6 +349,8 @@ __global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint3
     double *sv = smem + (size_t)warp * p.E;
     const uint32_t stride = gridDim.x * kWarps;
     uint32_t t = blockIdx.x * kWarps + warp;
+    pdl_launch_dependents();
+    pdl_wait_prior();
     if (t >= p.T) return;
     float bias[PER], zn[PER];
 #pragma unroll
@@ -468,12 +472,12 @@ template <bool F16> cudaError_t launch_fast(const Params &p, uint32_t per, uint3
     const unsigned grid = want < most ? want : most;
     const size_t smem = group_lanes ? (size_t)kWarps * p.E * sizeof(double) : 0;
     switch (per) {
-#define GATE_CASE(N) case N: fast_kernel<N, F16><<<grid, 32 * kWarps, smem, st>>>(p, group_lanes); break;
+#define GATE_CASE(N) case N: return launch_overlapped(fast_kernel<N, F16>, dim3(grid), dim3(32 * kWarps), smem, st, p, group_lanes);
     GATE_CASE(1) GATE_CASE(2) GATE_CASE(3) GATE_CASE(4) GATE_CASE(5) GATE_CASE(6) GATE_CASE(8) GATE_CASE(10) GATE_CASE(12)
     GATE_CASE(16)
 #undef GATE_CASE
     }
-    return cudaGetLastError();
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace gate
@@ -502,11 +506,8 @@ cudaError_t launch_moe_gate(const GateLaunch &L, cudaStream_t st)
     }
     const unsigned grid = (L.T + kWarps - 1) / kWarps;
     const size_t smem = (size_t)kWarps * L.E * sizeof(double);
-    if (L.E <= 64) any_kernel<2><<<grid, 32 * kWarps, smem, st>>>(p);
-    else if (L.E <= 128) any_kernel<4><<<grid, 32 * kWarps, smem, st>>>(p);
-    else if (L.E <= 256) any_kernel<8><<<grid, 32 * kWarps, smem, st>>>(p);
-    else any_kernel<16><<<grid, 32 * kWarps, smem, st>>>(p);
-    return cudaGetLastError();
+    return launch_overlapped(L.E <= 64 ? any_kernel<2> : L.E <= 128 ? any_kernel<4> : L.E <= 256 ? any_kernel<8> : any_kernel<16>,
+                             dim3(grid), dim3(32 * kWarps), smem, st, p);
 }
 
 }  // namespace mpp41
