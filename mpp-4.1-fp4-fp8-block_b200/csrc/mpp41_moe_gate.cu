@@ -52,8 +52,19 @@ constexpr float kTol = 1.0f / 524288.0f;
 
 template <typename F> struct Num;
 template <> struct Num<float> {
-    static __device__ __forceinline__ float exp(float x) { return __expf(x); }
-    static __device__ __forceinline__ float rcp(float x) { return __fdividef(1.0f, x); }
+    // hardware exponential and reciprocal (2 ulp and 1 ulp), results below 2^-126 as 0
+    static __device__ __forceinline__ float exp(float x)
+    {
+        float r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+        return r;
+    }
+    static __device__ __forceinline__ float rcp(float x)
+    {
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+        return r;
+    }
     static __device__ __forceinline__ float inf() { return INFINITY; }
 };
 template <> struct Num<double> {
@@ -206,24 +217,26 @@ __device__ __noinline__ uint32_t exact_token(const Params &p, size_t row, uint32
     return e;
 }
 
-// Weight of the lane's chosen expert e (lanes below k). zmax and zsum: softmax's
-// maximum and sum over all experts, used without renormalisation.
-__device__ __forceinline__ void write_slot(const Params &p, size_t t, uint32_t lane, uint32_t e, float zmax, float zsum)
+// Weight of the lane's chosen expert e: lanes come in runs of kp (a power of two, at least
+// k), one run a token t, the lane's slot in it s. zmax and zsum: softmax's maximum and
+// sum over all experts, used without renormalisation. live: the run has a token.
+__device__ __forceinline__ void write_slot(const Params &p, size_t t, uint32_t s, uint32_t kp, bool live, uint32_t e, float zmax,
+                                           float zsum)
 {
-    const bool have = lane < p.k;
+    const bool have = live && s < p.k;
     const float zc = have ? load_logit(p, t * p.E + e) : -INFINITY;
     float w = 0.0f, sum;
     if (p.renorm) {
         // relative to the largest chosen logit, so that scores too small for fp32 keep their ratio
-        const float m = warp_max(zc);
+        float m = zc;
+        for (uint32_t o = kp >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
         const bool low = !p.sigmoid || m < 0.0f;
         if (zc > -INFINITY) {
             w = low ? (zc == m ? 1.0f : expf(zc - m)) : 1.0f;
             if (p.sigmoid) w = __fdiv_rn(w, 1.0f + (low ? expf(zc) : expf(-zc)));
         }
         sum = w;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+        for (uint32_t o = kp >> 1; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
     } else if (p.sigmoid) {
         w = __fdiv_rn(1.0f, 1.0f + expf(-zc));
         sum = 1.0f;
@@ -232,8 +245,8 @@ __device__ __forceinline__ void write_slot(const Params &p, size_t t, uint32_t l
         sum = zsum;
     }
     if (have) {
-        p.ids[t * p.k + lane] = (int32_t)e;
-        p.weights[t * p.k + lane] = sum > 0.0f ? __fdiv_rn(w, sum) * p.scale : 0.0f;
+        p.ids[t * p.k + s] = (int32_t)e;
+        p.weights[t * p.k + s] = sum > 0.0f ? __fdiv_rn(w, sum) * p.scale : 0.0f;
     }
 }
 
@@ -269,7 +282,7 @@ __global__ void __launch_bounds__(32 * kWarps) any_kernel(const Params p)
     if (!choose<float, PER>(p, z, lane, reinterpret_cast<float *>(sv), e)) choose<double, PER>(p, z, lane, sv, e);
     float m = 0.0f, sum = 1.0f;
     if (!p.renorm && !p.sigmoid) softmax_norm<PER>(z, m, sum);
-    write_slot(p, t, lane, e, m, sum);
+    write_slot(p, t, lane, 32, true, e, m, sum);
 }
 
 // Order-preserving bits of a float (not NaN); never 0.
@@ -335,144 +348,161 @@ __device__ __forceinline__ void load_lane(const Params &p, uint32_t t, uint32_t 
     }
 }
 
-// group_lanes: lanes a group takes (a
-// power of two) where groups are dropped, else 0.
+// group_lanes: lanes a group takes (a power of two) where groups are dropped, else 0.
+// A warp chooses for `batch` tokens, one after the other, and then weighs their choices
+// together, kp lanes a token (batch * kp <= 32).
 template <int PER, bool F16>
-__global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint32_t group_lanes)
+__global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint32_t group_lanes, uint32_t batch, uint32_t kp)
 {
     extern __shared__ double smem[];
     __shared__ uint32_t sel[kWarps][32];
+    __shared__ float2 norm[kWarps][32];
     constexpr int kBits = key_bits(PER);
     constexpr uint32_t kLow = (1u << kBits) - 1u;
     constexpr int kExactPer = PER <= 2 ? 2 : PER <= 4 ? 4 : PER <= 8 ? 8 : 16;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double *sv = smem + (size_t)warp * p.E;
-    const uint32_t stride = gridDim.x * kWarps;
-    uint32_t t = blockIdx.x * kWarps + warp;
+    const uint32_t stride = gridDim.x * kWarps * batch;
     pdl_launch_dependents();
     pdl_wait_prior();
-    if (t >= p.T) return;
-    float bias[PER], zn[PER];
+    float bias[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) bias[j] = p.bias && lane * PER + j < p.E ? p.bias[lane * PER + j] : 0.0f;
-    load_lane<PER, F16>(p, t, lane, zn);
+    for (int j = 0; j < PER; ++j) {
+        bias[j] = p.bias && lane * PER + j < p.E ? p.bias[lane * PER + j] : 0.0f;
+        if (!(bias[j] > -INFINITY)) bias[j] = -INFINITY;   // NaN: as a masked expert
+    }
     // what two compared values may be off by together, beside the keys' cut bits:
     // fp32 scores, or nothing where the logits are compared
     const float tol = p.by_logit ? 0.0f : p.sigmoid ? 1.0f / 1048576.0f : 1.0f / 262144.0f;
     const float cut = (float)(2u << kBits) / 8388608.0f;
     const bool check = !(p.by_logit && F16);   // fp16 logits lose no bits to the position
-    for (; t < p.T; t += stride) {
-        float z[PER], v[PER];
+    for (uint64_t t0 = (uint64_t)(blockIdx.x * kWarps + warp) * batch; t0 < p.T; t0 += stride) {
+        const uint32_t n = (uint32_t)min((uint64_t)batch, p.T - t0);
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t t = (uint32_t)t0 + i;
+            float z[PER], v[PER];
+            load_lane<PER, F16>(p, t, lane, z);
+            if (p.by_logit) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) z[j] = zn[j] > -INFINITY ? zn[j] + 0.0f : -INFINITY;   // NaN masks; -0 -> +0
-        if (t + stride < p.T) load_lane<PER, F16>(p, t + stride, lane, zn);
-        float zm = 0.0f, zsum = 1.0f;
-        if (p.by_logit) {
+                for (int j = 0; j < PER; ++j) v[j] = z[j] > -INFINITY ? z[j] + 0.0f : -INFINITY;   // NaN masks; -0 -> +0
+            } else if (p.sigmoid) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) v[j] = z[j];
-        } else {
-            if (p.sigmoid) {
-#pragma unroll
-                for (int j = 0; j < PER; ++j) v[j] = Num<float>::rcp(1.0f + Num<float>::exp(-z[j]));
+                for (int j = 0; j < PER; ++j) {
+                    v[j] = Num<float>::rcp(1.0f + Num<float>::exp(-z[j])) + bias[j];
+                    if (!(z[j] > -INFINITY)) v[j] = -INFINITY;
+                }
             } else {
-                zm = z[0];
+                float m = z[0];
 #pragma unroll
-                for (int j = 1; j < PER; ++j) zm = fmaxf(zm, z[j]);
-                zm = warp_max(zm);
+                for (int j = 1; j < PER; ++j) m = fmaxf(m, z[j]);   // NaN is no maximum
+                m = warp_max(m > -INFINITY ? m : -INFINITY);
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    v[j] = z[j] == zm ? 1.0f : Num<float>::exp(z[j] - zm);
+                    v[j] = z[j] == m ? 1.0f : Num<float>::exp(z[j] - m);
                     if (!(z[j] > -INFINITY)) v[j] = 0.0f;
                     sum += v[j];
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-                const float r = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+                const float r = sum > 0.0f ? Num<float>::rcp(sum) : 0.0f;
 #pragma unroll
-                for (int j = 0; j < PER; ++j) v[j] *= r;
+                for (int j = 0; j < PER; ++j) {
+                    v[j] = v[j] * r + bias[j];
+                    if (!(z[j] > -INFINITY)) v[j] = -INFINITY;
+                }
             }
+            bool sure = true, keep = lane * PER < p.E;
+            if (group_lanes) {
+                float b0 = v[0], b1 = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                v[j] += bias[j];
-                v[j] = z[j] > -INFINITY && v[j] > -INFINITY ? v[j] + 0.0f : -INFINITY;   // NaN too
+                for (int j = 1; j < PER; ++j) {
+                    b1 = fmaxf(b1, fminf(b0, v[j]));
+                    b0 = fmaxf(b0, v[j]);
+                }
+                for (uint32_t o = group_lanes >> 1; o; o >>= 1) {
+                    const float o0 = __shfl_xor_sync(kFull, b0, o), o1 = __shfl_xor_sync(kFull, b1, o);
+                    b1 = fmaxf(fminf(b0, o0), fmaxf(b1, o1));
+                    b0 = fmaxf(b0, o0);
+                }
+                const float worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
+                const uint32_t mine = lane / group_lanes;
+                uint32_t rank = 0;
+                for (uint32_t g = 0; g < p.groups; ++g) {
+                    const float w = __shfl_sync(kFull, worth, g * group_lanes);
+                    rank += w > worth || (w == worth && g < mine) ? 1u : 0u;
+                }
+                const bool real = mine < p.groups;
+                keep = real && rank < p.top_groups;
+                if (!p.by_logit) {
+                    // the last group that stays and the first that goes have to be well apart
+                    const uint32_t k = order_bits(worth);
+                    const float in = order_value(__reduce_min_sync(kFull, keep ? k : 0xFFFFFFFFu));
+                    const float out = order_value(__reduce_max_sync(kFull, real && !keep ? k : 0u));
+                    sure = in - out > 2.0f * tol * (1.0f + fabsf(in));
+                }
             }
-        }
-        bool sure = true, keep = lane * PER < p.E;
-        if (group_lanes) {
-            float b0 = v[0], b1 = -INFINITY;
+            uint32_t key[PER];
 #pragma unroll
-            for (int j = 1; j < PER; ++j) {
-                b1 = fmaxf(b1, fminf(b0, v[j]));
-                b0 = fmaxf(b0, v[j]);
-            }
-            for (uint32_t o = group_lanes >> 1; o; o >>= 1) {
-                const float o0 = __shfl_xor_sync(kFull, b0, o), o1 = __shfl_xor_sync(kFull, b1, o);
-                b1 = fmaxf(fminf(b0, o0), fmaxf(b1, o1));
-                b0 = fmaxf(b0, o0);
-            }
-            const float worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
-            const uint32_t mine = lane / group_lanes;
-            uint32_t rank = 0;
-            for (uint32_t g = 0; g < p.groups; ++g) {
-                const float w = __shfl_sync(kFull, worth, g * group_lanes);
-                rank += w > worth || (w == worth && g < mine) ? 1u : 0u;
-            }
-            const bool real = mine < p.groups;
-            keep = real && rank < p.top_groups;
-            if (!p.by_logit) {
-                // the last group that stays and the first that goes have to be well apart
-                const uint32_t k = order_bits(worth);
-                const float in = order_value(__reduce_min_sync(kFull, keep ? k : 0xFFFFFFFFu));
-                const float out = order_value(__reduce_max_sync(kFull, real && !keep ? k : 0u));
-                sure = in - out > 2.0f * tol * (1.0f + fabsf(in));
-            }
-        }
-        uint32_t key[PER];
+            for (int j = 0; j < PER; ++j)
+                key[j] = keep && lane * PER + j < p.E ? (order_bits(v[j]) & ~kLow) | (kLow - (uint32_t)j) : 0u;
+            sort_desc<PER>(key);
+            uint32_t won = 0;   // lane s: the winning key of round s
+            for (uint32_t s = 0; s < p.k; ++s) {
+                const uint32_t m = __reduce_max_sync(kFull, key[0]);
+                // equal but for the position: the lowest lane has the lowest expert
+                const uint32_t first = __ffs(__ballot_sync(kFull, (key[0] >> kBits) == (m >> kBits))) - 1;
+                const bool win = lane == first;
+                if (lane == s) won = m;
+                if (win) sel[warp][i * kp + s] = lane * PER + (kLow - (key[0] & kLow));
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-            key[j] = keep && lane * PER + j < p.E ? (order_bits(v[j]) & ~kLow) | (kLow - (uint32_t)j) : 0u;
-        sort_desc<PER>(key);
-        uint32_t won = 0;   // lane s: the winning key of round s
-        for (uint32_t s = 0; s < p.k; ++s) {
-            const uint32_t m = __reduce_max_sync(kFull, key[0]);
-            // equal but for the position: the lowest lane has the lowest expert
-            const uint32_t first = __ffs(__ballot_sync(kFull, (key[0] >> kBits) == (m >> kBits))) - 1;
-            if (lane == s) won = m;
-            if (lane == first) {
-                sel[warp][s] = lane * PER + (kLow - (key[0] & kLow));
-#pragma unroll
-                for (int j = 0; j + 1 < PER; ++j) key[j] = key[j + 1];
-                key[PER - 1] = 0u;
+                for (int j = 0; j + 1 < PER; ++j) key[j] = win ? key[j + 1] : key[j];
+                if (win) key[PER - 1] = 0u;
             }
-        }
-        if (check) {
-            // neighbours in the order, the first not chosen among them, have to be apart
-            const uint32_t after = __reduce_max_sync(kFull, key[0]);
-            uint32_t next = __shfl_down_sync(kFull, won, 1);
-            if (lane + 1 == p.k) next = after;
-            if (lane < p.k && next != 0u) {
-                const float a = order_value(won | kLow), b = order_value(next | kLow);
-                sure = sure && a - b > 2.0f * tol + fmaxf(fabsf(a), fabsf(b)) * (cut + 2.0f * tol);
+            if (check) {
+                // neighbours in the order, the first not chosen among them, have to be apart
+                const uint32_t after = __reduce_max_sync(kFull, key[0]);
+                uint32_t next = __shfl_down_sync(kFull, won, 1);
+                if (lane + 1 == p.k) next = after;
+                if (lane < p.k && next != 0u) {
+                    const float a = order_value(won | kLow), b = order_value(next | kLow);
+                    sure = sure && a - b > 2.0f * tol + fmaxf(fabsf(a), fabsf(b)) * (cut + 2.0f * tol);
+                }
+                if (!__all_sync(kFull, sure)) {
+                    __syncwarp();
+                    const uint32_t e = exact_token<kExactPer>(p, (size_t)t * p.E, lane, sv);
+                    if (lane < p.k) sel[warp][i * kp + lane] = e;
+                }
+            }
+            if (!p.renorm && !p.sigmoid) {
+                float m, sum;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) z[j] = z[j] > -INFINITY ? z[j] : -INFINITY;
+                softmax_norm<PER>(z, m, sum);
+                if (lane == 0) norm[warp][i] = make_float2(m, sum);
             }
         }
         __syncwarp();
-        uint32_t e = lane < p.k ? sel[warp][lane] : 0u;
-        if (!__all_sync(kFull, sure)) e = exact_token<kExactPer>(p, (size_t)t * p.E, lane, sv);
-        if (!p.renorm && !p.sigmoid) softmax_norm<PER>(z, zm, zsum);
-        write_slot(p, t, lane, e, zm, zsum);
+        const uint32_t i = lane / kp, s = lane % kp;
+        const bool live = i < n;
+        const float2 nm = live ? norm[warp][i] : make_float2(0.0f, 1.0f);
+        write_slot(p, t0 + i, s, kp, live, live && s < p.k ? sel[warp][i * kp + s] : 0u, nm.x, nm.y);
         __syncwarp();
     }
 }
 
 template <bool F16> cudaError_t launch_fast(const Params &p, uint32_t per, uint32_t group_lanes, cudaStream_t st)
 {
-    // a warp keeps bias and the next token's logits in registers: no more CTAs than run at once
-    const uint32_t want = (p.T + kWarps - 1) / kWarps, most = 148 * 8;
-    const unsigned grid = want < most ? want : most;
+    // Weighing a token's k choices leaves most lanes idle: from enough tokens for every
+    // warp slot, a warp weighs as many together as fit its lanes.
+    uint32_t kp = 1;
+    while (kp < p.k) kp *= 2;
+    const uint32_t most = 148 * 8, batch = p.T >= most * kWarps ? 32 / kp : 1;
+    const uint64_t per_cta = (uint64_t)kWarps * batch, want = (p.T + per_cta - 1) / per_cta;
+    const unsigned grid = (unsigned)(want < most ? want : most);
     const size_t smem = group_lanes ? (size_t)kWarps * p.E * sizeof(double) : 0;
     switch (per) {
-#define GATE_CASE(N) case N: return launch_overlapped(fast_kernel<N, F16>, dim3(grid), dim3(32 * kWarps), smem, st, p, group_lanes);
+#define GATE_CASE(N) case N: return launch_overlapped(fast_kernel<N, F16>, dim3(grid), dim3(32 * kWarps), smem, st, p, group_lanes, batch, kp);
     GATE_CASE(1) GATE_CASE(2) GATE_CASE(3) GATE_CASE(4) GATE_CASE(5) GATE_CASE(6) GATE_CASE(8) GATE_CASE(10) GATE_CASE(12)
     GATE_CASE(16)
 #undef GATE_CASE

@@ -81,6 +81,7 @@ def test_quantize_weights(ctx, fmt, n, k):
     rng = np.random.default_rng(n + k)
     w = (rng.standard_normal((n, k)) * 0.02).astype(np.float32)
     w[: min(n, 128), : min(k, 128)] *= 0 if n > 200 else 1
+    w[128:256, : min(k, 128)] *= np.float32(1e-36)          # maxima that qmax / amax would overflow for
     q = torch.zeros(n, k, dtype=torch.uint8, device="cuda")
     s = torch.zeros(F.up(n), F.up(k), device="cuda")
     ctx.quantize_weights_fp8(F.FMT[fmt], torch.from_numpy(w).cuda(), n, k, q, s)
@@ -90,7 +91,8 @@ def test_quantize_weights(ctx, fmt, n, k):
     blk = pad.reshape(F.up(n), 128, F.up(k), 128)
     amax = np.abs(blk).max(axis=(1, 3))
     safe = np.where(amax > 0, amax, np.float32(1))
-    v = (blk / safe[:, None, :, None]) * np.float32(F.QMAX[fmt])
+    by, qmax = safe[:, None, :, None], np.float32(F.QMAX[fmt])
+    v = np.where(by < np.float32(1e-30), (blk / by) * qmax, blk * (qmax / np.maximum(by, np.float32(1e-30))))
     rq = F.nearest8(v.astype(np.float64), fmt).reshape(pad.shape)[:n, :k]
     assert np.array_equal(F.from_fp8(q, fmt), rq)
     assert np.array_equal(s.cpu().numpy(), np.where(amax > 0, amax / np.float32(F.QMAX[fmt]), np.float32(1)))
