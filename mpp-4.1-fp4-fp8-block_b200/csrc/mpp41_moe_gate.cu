@@ -9,17 +9,17 @@
 // The selection is exact: it is the one the 64-bit values give. Without a bias
 // (and without sums of two scores) v is monotone in the logit, so the logits are
 // compared themselves. Otherwise fp32 scores decide, and wherever two values that
-// the outcome depends on lie closer than the fp32 error, that warp computes the
-// token again in 64 bits (exact_token): a few tokens in a thousand for scores of a
-// trained router's spread, which costs less than 64-bit exponentials for all.
+// the outcome depends on lie closer than the fp32 error, that warp decides the
+// token again in 64 bits (exact_token, about 3 us): a few tokens in a thousand for
+// scores of a trained router's spread.
 //
 // fast_kernel: a lane holds PER neighbouring experts (16-byte loads), sorted once by
 // 32-bit keys that carry the position in their lowest bits; each of the k rounds is
 // then one warp-wide maximum of the lanes' heads and a shift in the winner's lane.
 // A group is a run of lanes, its two best a butterfly. 32768 tokens of 256 experts are
 // bound by instruction issue, not by the 34 MB they read.
-// any_kernel (every token through the exact comparison in fp32, then 64 bits where
-// needed) takes the group sizes that do not fall on lane borders.
+// any_kernel (every token through exact_token) takes the group sizes that do not fall
+// on lane borders.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -45,33 +45,20 @@ struct Params {
     float scale;
 };
 
-// fp32 fast exponentials: the scores' absolute error is below 2^-20 (a sigmoid's
-// slope times the exponent's error peaks at 0.25 * 2^-20, a softmax value's at
-// 0.37 * 2^-20 plus its sum's); sums with a bias add half an ulp of |v|.
-constexpr float kTol = 1.0f / 524288.0f;
+// Hardware exponential and reciprocal (2 ulp and 1 ulp), results below 2^-126 as 0.
+__device__ __forceinline__ float fast_exp(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
 
-template <typename F> struct Num;
-template <> struct Num<float> {
-    // hardware exponential and reciprocal (2 ulp and 1 ulp), results below 2^-126 as 0
-    static __device__ __forceinline__ float exp(float x)
-    {
-        float r;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
-        return r;
-    }
-    static __device__ __forceinline__ float rcp(float x)
-    {
-        float r;
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-        return r;
-    }
-    static __device__ __forceinline__ float inf() { return INFINITY; }
-};
-template <> struct Num<double> {
-    static __device__ __forceinline__ double exp(double x) { return ::exp(x); }
-    static __device__ __forceinline__ double rcp(double x) { return 1.0 / x; }
-    static __device__ __forceinline__ double inf() { return (double)INFINITY; }
-};
+__device__ __forceinline__ float fast_rcp(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 __device__ __forceinline__ float load_logit(const Params &p, size_t at)
 {
@@ -89,132 +76,114 @@ template <typename F> __device__ __forceinline__ F warp_max(F v)
     return v;
 }
 
-// Exact comparisons in layout expert = lane + 32 j. The token's chosen experts: lane s < k gets the expert of slot s. Returns whether
-// the choice holds for the exact values (always for F = double).
-template <typename F, int PER>
-__device__ __forceinline__ bool choose(const Params &p, const float (&z)[PER], uint32_t lane, F *sv, uint32_t &mine)
+// Order-preserving bits of a double (not NaN); never 0.
+__device__ __forceinline__ unsigned long long order_bits64(double v)
 {
-    const F inf = Num<F>::inf();
-    F v[PER];
-    if (p.by_logit) {
+    const long long u = __double_as_longlong(v);
+    return (unsigned long long)(u ^ ((u >> 63) | (long long)0x8000000000000000ull));
+}
+
+// One token decided in 64 bits, experts lane + 32 j, j < PER. sv: E doubles of shared
+// memory where groups are dropped. Lane s < k returns the expert of slot s. Built for
+// latency (about 2 us): a token that comes here holds up its warp's others.
+template <int PER>
+__device__ __noinline__ uint32_t exact_token(const Params &p, size_t row, uint32_t lane, double *sv)
+{
+    const double inf = (double)INFINITY;
+    double v[PER];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = (F)z[j];
-    } else {
+    for (int j = 0; j < PER; ++j) v[j] = lane + 32 * j < p.E ? (double)load_logit(p, row + lane + 32 * j) : -inf;
+    if (!p.by_logit) {
+        uint32_t masked = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) masked |= v[j] > -inf ? 0u : 1u << j;
         if (p.sigmoid) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) v[j] = Num<F>::rcp((F)1 + Num<F>::exp(-(F)z[j]));
+            for (int j = 0; j < PER; ++j) v[j] = 1.0 / (1.0 + exp(-v[j]));
         } else {
-            float zm = z[0];
+            double m = v[0], sum = 0.0;
 #pragma unroll
-            for (int j = 1; j < PER; ++j) zm = fmaxf(zm, z[j]);
-            zm = warp_max(zm);
-            F sum = 0;
+            for (int j = 1; j < PER; ++j) m = fmax(m, v[j]);
+            m = warp_max(m);
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                v[j] = z[j] == zm ? (F)1 : Num<F>::exp((F)z[j] - (F)zm);
-                if (z[j] == -INFINITY) v[j] = 0;
+                v[j] = masked >> j & 1u ? 0.0 : (v[j] == m ? 1.0 : exp(v[j] - m));
                 sum += v[j];
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-            const F r = sum > (F)0 ? (F)1 / sum : (F)0;
+            sum = sum > 0.0 ? sum : 1.0;
 #pragma unroll
-            for (int j = 0; j < PER; ++j) v[j] *= r;
+            for (int j = 0; j < PER; ++j) v[j] /= sum;
         }
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const uint32_t e = lane + 32 * j;
-            if (p.bias && e < p.E) v[j] += (F)p.bias[e];
-            if (!(z[j] > -INFINITY) || !(v[j] == v[j])) v[j] = -inf;
-            v[j] += (F)0;
+            if (p.bias && lane + 32 * j < p.E) v[j] += (double)p.bias[lane + 32 * j];
+            if (masked >> j & 1u || !(v[j] == v[j])) v[j] = -inf;
         }
     }
-    bool sure = true;
-    const bool check = sizeof(F) == 4 && !p.by_logit;
     uint32_t keep = kFull;   // groups that stay
     if (p.top_groups < p.groups) {
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             if (lane + 32 * j < p.E) sv[lane + 32 * j] = v[j];
         __syncwarp();
-        // lane g: the two largest of group g (groups <= 32)
-        F b0 = -inf, b1 = -inf;
-        if (lane < p.groups) {
-            const F *s = sv + lane * p.group_size;
-            uint32_t at = lane % p.group_size;   // start apart: groups of a power of two share a bank
-            for (uint32_t i = 0; i < p.group_size; ++i) {
-                const F x = s[at];
-                at = at + 1 == p.group_size ? 0 : at + 1;
-                b1 = x > b0 ? b0 : (x > b1 ? x : b1);
-                b0 = x > b0 ? x : b0;
+        // the two largest of each group: `lanes` lanes a group (a power of two), each
+        // taking every lanes-th of its experts
+        uint32_t lanes = 32;
+        while (lanes * p.groups > 32 && lanes > 1) lanes >>= 1;
+        const uint32_t g = lane / lanes, sub = lane % lanes;
+        double b0 = -inf, b1 = -inf;
+        if (g < p.groups)
+            for (uint32_t i = sub; i < p.group_size; i += lanes) {
+                const double x = sv[g * p.group_size + i];
+                b1 = fmax(b1, fmin(b0, x));
+                b0 = fmax(b0, x);
             }
+        for (uint32_t o = lanes >> 1; o; o >>= 1) {
+            const double o0 = __shfl_xor_sync(kFull, b0, o), o1 = __shfl_xor_sync(kFull, b1, o);
+            b1 = fmax(fmin(b0, o0), fmax(b1, o1));
+            b0 = fmax(b0, o0);
         }
-        __syncwarp();
-        const F worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
+        const double worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
         uint32_t rank = 0;
-        F edge = inf;   // distance to the nearest group on the other side of the cut
-        for (uint32_t g = 0; g < p.groups; ++g) {
-            const F w = __shfl_sync(kFull, worth, g);
-            if (w > worth || (w == worth && g < lane)) ++rank;
+#pragma unroll 4
+        for (uint32_t i = 0; i < p.groups; ++i) {
+            const double w = __shfl_sync(kFull, worth, i * lanes);
+            rank += w > worth || (w == worth && i < g) ? 1u : 0u;
         }
-        const bool in = lane < p.groups && rank < p.top_groups;
-        keep = __ballot_sync(kFull, in);
-        if (check) {
-            const uint32_t last = __ballot_sync(kFull, lane < p.groups && rank == p.top_groups - 1);
-            const uint32_t next = __ballot_sync(kFull, lane < p.groups && rank == p.top_groups);
-            const F a = __shfl_sync(kFull, worth, __ffs(last) - 1), b = __shfl_sync(kFull, worth, __ffs(next) - 1);
-            edge = a - b;
-            sure = edge > (F)(2 * kTol) * ((F)1 + (a < 0 ? -a : a));
-        }
+        const uint32_t in = __ballot_sync(kFull, g < p.groups && rank < p.top_groups);
+        keep = 0u;   // bit g from its first lane
+        for (uint32_t i = 0; i < p.groups; ++i) keep |= (in >> (i * lanes) & 1u) << i;
+        __syncwarp();
     }
-    // repeated arg-max; taken and dropped experts leave through `open`
-    uint32_t open = 0;
+    // repeated arg-max by 64-bit keys: upper half, lower half, then the lowest expert; 0 = not open
+    unsigned long long key[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const uint32_t e = lane + 32 * j;
-        if (e < p.E && (keep == kFull || keep >> (e / p.group_size) & 1u)) open |= 1u << j;
+        key[j] = e < p.E && (keep == kFull || keep >> (e / p.group_size) & 1u) ? order_bits64(v[j] + 0.0) : 0ull;
     }
-    F before = inf;
-    const uint32_t rounds = check ? p.k + 1 : p.k;
-    for (uint32_t s = 0; s < rounds; ++s) {
-        F bv = -inf;
-        uint32_t be = 0xffffffffu;
+    uint32_t mine = 0;
+    for (uint32_t s = 0; s < p.k; ++s) {
+        unsigned long long h = key[0];
+#pragma unroll
+        for (int j = 1; j < PER; ++j) h = key[j] > h ? key[j] : h;
+        const uint32_t hi = __reduce_max_sync(kFull, (uint32_t)(h >> 32));
+        const uint32_t lo = __reduce_max_sync(kFull, (uint32_t)(h >> 32) == hi ? (uint32_t)h : 0u);
+        const unsigned long long m = (unsigned long long)hi << 32 | lo;
+        uint32_t e = kFull;
+#pragma unroll
+        for (int j = PER - 1; j >= 0; --j) e = key[j] == m ? lane + 32 * j : e;
+        e = __reduce_min_sync(kFull, e);
+        if (lane == s) mine = e;
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            if (open >> j & 1u && (v[j] > bv || be == 0xffffffffu)) {
-                bv = v[j];
-                be = lane + 32 * j;
-            }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const F ov = __shfl_xor_sync(kFull, bv, o);
-            const uint32_t oe = __shfl_xor_sync(kFull, be, o);
-            if (oe != 0xffffffffu && (be == 0xffffffffu || ov > bv || (ov == bv && oe < be))) {
-                bv = ov;
-                be = oe;
-            }
-        }
-        if (be == 0xffffffffu) break;   // only the extra round can run out of experts
-        if (check && s) sure = sure && (before - bv > (F)(2 * kTol) * ((F)1 + (bv < 0 ? -bv : bv)));
-        before = bv;
-        if (s < p.k) {
-            if (lane == s) mine = be;
-            if (be % 32 == lane) open &= ~(1u << (be / 32));
-        }
+            if (lane + 32 * j == e) key[j] = 0ull;
     }
-    return sure;
-}
-
-// One token decided exactly; sv: E doubles of shared memory where groups are dropped.
-template <int PER>
-__device__ __noinline__ uint32_t exact_token(const Params &p, size_t row, uint32_t lane, double *sv)
-{
-    float z[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) z[j] = lane + 32 * j < p.E ? load_logit(p, row + lane + 32 * j) : -INFINITY;
-    uint32_t e = 0;
-    if (!p.by_logit || !choose<float, PER>(p, z, lane, reinterpret_cast<float *>(sv), e)) choose<double, PER>(p, z, lane, sv, e);
-    return e;
+    __syncwarp();
+    return mine;
 }
 
 // Weight of the lane's chosen expert e: lanes come in runs of kp (a power of two, at least
@@ -269,19 +238,22 @@ __global__ void __launch_bounds__(32 * kWarps) any_kernel(const Params p)
 {
     extern __shared__ double smem[];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double *sv = smem + (size_t)warp * p.E;
     const uint32_t t = blockIdx.x * kWarps + warp;
     pdl_launch_dependents();
     pdl_wait_prior();
     if (t >= p.T) return;
     const size_t row = (size_t)t * p.E;
-    float z[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) z[j] = lane + 32 * j < p.E ? load_logit(p, row + lane + 32 * j) : -INFINITY;
-    uint32_t e = 0;
-    if (!choose<float, PER>(p, z, lane, reinterpret_cast<float *>(sv), e)) choose<double, PER>(p, z, lane, sv, e);
-    float m = 0.0f, sum = 1.0f;
-    if (!p.renorm && !p.sigmoid) softmax_norm<PER>(z, m, sum);
+    const uint32_t e = exact_token<PER>(p, row, lane, smem + (size_t)warp * p.E);
+    float m = -INFINITY, sum = 0.0f;
+    if (!p.renorm && !p.sigmoid) {
+        for (uint32_t i = lane; i < p.E; i += 32) m = fmaxf(m, load_logit(p, row + i));
+        m = warp_max(m);
+        for (uint32_t i = lane; i < p.E; i += 32) {
+            const float z = load_logit(p, row + i);
+            sum += z > -INFINITY ? (z == m ? 1.0f : expf(z - m)) : 0.0f;
+        }
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    }
     write_slot(p, t, lane, 32, true, e, m, sum);
 }
 
@@ -352,7 +324,7 @@ __device__ __forceinline__ void load_lane(const Params &p, uint32_t t, uint32_t 
 // A warp chooses for `batch` tokens, one after the other, and then weighs their choices
 // together, kp lanes a token (batch * kp <= 32).
 template <int PER, bool F16>
-__global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint32_t group_lanes, uint32_t batch, uint32_t kp)
+__global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(const Params p, uint32_t group_lanes, uint32_t batch, uint32_t kp)
 {
     extern __shared__ double smem[];
     __shared__ uint32_t sel[kWarps][32];
@@ -371,10 +343,16 @@ __global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint3
         bias[j] = p.bias && lane * PER + j < p.E ? p.bias[lane * PER + j] : 0.0f;
         if (!(bias[j] > -INFINITY)) bias[j] = -INFINITY;   // NaN: as a masked expert
     }
-    // what two compared values may be off by together, beside the keys' cut bits:
-    // fp32 scores, or nothing where the logits are compared
-    const float tol = p.by_logit ? 0.0f : p.sigmoid ? 1.0f / 1048576.0f : 1.0f / 262144.0f;
-    const float cut = (float)(2u << kBits) / 8388608.0f;
+    // How far two fp32 values have to be apart for their order to be the exact values'.
+    // A score: ex2 (2^-22 of its value, and |x| 2^-24 by its argument) times the sigmoid's
+    // slope or the softmax value stays below 2^-24 * 1.3, the sum 1 + e, the reciprocal and
+    // the bias add half, one and half an ulp: below 2^-22 for values up to 2, both together
+    // 2^-21 (and 2^-23 |v| for larger ones). A softmax's sum is off by one factor for all,
+    // at most PER + 10 half ulps. Logits compared themselves have no error. Keys cut to
+    // their upper bits keep the order; equal ones are less than one cut unit apart.
+    const float tol = p.by_logit ? 0.0f : (p.sigmoid ? 0.0f : (float)(PER + 10) / 16777216.0f) + 1.0f / 2097152.0f;
+    const float unit = ((float)(1u << kBits) + (p.by_logit ? 0.0f : 1.0f)) / 8388608.0f;
+    const bool ragged = p.E % PER != 0;
     const bool check = !(p.by_logit && F16);   // fp16 logits lose no bits to the position
     for (uint64_t t0 = (uint64_t)(blockIdx.x * kWarps + warp) * batch; t0 < p.T; t0 += stride) {
         const uint32_t n = (uint32_t)min((uint64_t)batch, p.T - t0);
@@ -388,7 +366,7 @@ __global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint3
             } else if (p.sigmoid) {
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    v[j] = Num<float>::rcp(1.0f + Num<float>::exp(-z[j])) + bias[j];
+                    v[j] = fast_rcp(1.0f + fast_exp(-z[j])) + bias[j];
                     if (!(z[j] > -INFINITY)) v[j] = -INFINITY;
                 }
             } else {
@@ -399,13 +377,13 @@ __global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint3
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
-                    v[j] = z[j] == m ? 1.0f : Num<float>::exp(z[j] - m);
+                    v[j] = z[j] == m ? 1.0f : fast_exp(z[j] - m);
                     if (!(z[j] > -INFINITY)) v[j] = 0.0f;
                     sum += v[j];
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-                const float r = sum > 0.0f ? Num<float>::rcp(sum) : 0.0f;
+                const float r = sum > 0.0f ? fast_rcp(sum) : 0.0f;
 #pragma unroll
                 for (int j = 0; j < PER; ++j) {
                     v[j] = v[j] * r + bias[j];
@@ -428,9 +406,15 @@ __global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint3
                 const float worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
                 const uint32_t mine = lane / group_lanes;
                 uint32_t rank = 0;
-                for (uint32_t g = 0; g < p.groups; ++g) {
-                    const float w = __shfl_sync(kFull, worth, g * group_lanes);
-                    rank += w > worth || (w == worth && g < mine) ? 1u : 0u;
+                if (p.by_logit) {
+                    for (uint32_t g = 0; g < p.groups; ++g) {
+                        const float w = __shfl_sync(kFull, worth, g * group_lanes);
+                        rank += w > worth || (w == worth && g < mine) ? 1u : 0u;
+                    }
+                } else {   // a tie at the cut is not sure anyway
+#pragma unroll 4
+                    for (uint32_t g = 0; g < p.groups; ++g)
+                        rank += __shfl_sync(kFull, worth, g * group_lanes) > worth ? 1u : 0u;
                 }
                 const bool real = mine < p.groups;
                 keep = real && rank < p.top_groups;
@@ -439,22 +423,31 @@ __global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint3
                     const uint32_t k = order_bits(worth);
                     const float in = order_value(__reduce_min_sync(kFull, keep ? k : 0xFFFFFFFFu));
                     const float out = order_value(__reduce_max_sync(kFull, real && !keep ? k : 0u));
-                    sure = in - out > 2.0f * tol * (1.0f + fabsf(in));
+                    sure = in - out > 2.0f * tol + fabsf(in) * (1.0f / 4194304.0f);   // sums of two
                 }
             }
             uint32_t key[PER];
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
-                key[j] = keep && lane * PER + j < p.E ? (order_bits(v[j]) & ~kLow) | (kLow - (uint32_t)j) : 0u;
+            for (int j = 0; j < PER; ++j) {
+                key[j] = keep ? (order_bits(v[j]) & ~kLow) | (kLow - (uint32_t)j) : 0u;
+                if (ragged && lane * PER + j >= p.E) key[j] = 0u;
+            }
             sort_desc<PER>(key);
-            uint32_t won = 0;   // lane s: the winning key of round s
+            uint32_t won = 0, pops = 0;   // lane s: the winning key of round s; heads this lane gave
+            uint32_t *out = &sel[warp][i * kp];
             for (uint32_t s = 0; s < p.k; ++s) {
                 const uint32_t m = __reduce_max_sync(kFull, key[0]);
-                // equal but for the position: the lowest lane has the lowest expert
-                const uint32_t first = __ffs(__ballot_sync(kFull, (key[0] >> kBits) == (m >> kBits))) - 1;
-                const bool win = lane == first;
+                bool win = key[0] == m;
+                if (!check) {
+                    // ties are exact here: the lowest lane has the lowest expert
+                    const uint32_t first = __ffs(__ballot_sync(kFull, (key[0] >> kBits) == (m >> kBits))) - 1;
+                    win = lane == first;
+                }
                 if (lane == s) won = m;
-                if (win) sel[warp][i * kp + s] = lane * PER + (kLow - (key[0] & kLow));
+                if (win) {
+                    out[s] = lane * PER + (kLow - (key[0] & kLow));
+                    ++pops;
+                }
 #pragma unroll
                 for (int j = 0; j + 1 < PER; ++j) key[j] = win ? key[j + 1] : key[j];
                 if (win) key[PER - 1] = 0u;
@@ -463,10 +456,11 @@ __global__ void __launch_bounds__(32 * kWarps) fast_kernel(const Params p, uint3
                 // neighbours in the order, the first not chosen among them, have to be apart
                 const uint32_t after = __reduce_max_sync(kFull, key[0]);
                 uint32_t next = __shfl_down_sync(kFull, won, 1);
+                sure = sure && __reduce_add_sync(kFull, pops) == p.k;   // two lanes with one key
                 if (lane + 1 == p.k) next = after;
                 if (lane < p.k && next != 0u) {
-                    const float a = order_value(won | kLow), b = order_value(next | kLow);
-                    sure = sure && a - b > 2.0f * tol + fmaxf(fabsf(a), fabsf(b)) * (cut + 2.0f * tol);
+                    const float a = order_value(won & ~kLow), b = order_value(next & ~kLow);
+                    sure = sure && (won >> kBits) != (next >> kBits) && a - b > tol + fmaxf(fabsf(a), fabsf(b)) * unit * (p.by_logit ? 0.0f : 1.0f);
                 }
                 if (!__all_sync(kFull, sure)) {
                     __syncwarp();
@@ -497,7 +491,7 @@ template <bool F16> cudaError_t launch_fast(const Params &p, uint32_t per, uint3
     // warp slot, a warp weighs as many together as fit its lanes.
     uint32_t kp = 1;
     while (kp < p.k) kp *= 2;
-    const uint32_t most = 148 * 8, batch = p.T >= most * kWarps ? 32 / kp : 1;
+    const uint32_t most = 148 * 7, batch = p.T >= most * kWarps ? 32 / kp : 1;
     const uint64_t per_cta = (uint64_t)kWarps * batch, want = (p.T + per_cta - 1) / per_cta;
     const unsigned grid = (unsigned)(want < most ? want : most);
     const size_t smem = group_lanes ? (size_t)kWarps * p.E * sizeof(double) : 0;
