@@ -239,10 +239,8 @@ mpp41_status mpp41_moe_fp8(mpp41_ctx *ctx, const mpp41_moe_fp8_desc *d, const vo
     auto f32 = [&](size_t at) { return reinterpret_cast<float *>(b + at); };
     int32_t *offsets = reinterpret_cast<int32_t *>(b + l.offsets), *inv = reinterpret_cast<int32_t *>(b + l.inv);
     cudaStream_t st = ctx->stream;
-    s = cuda_status(launch_fp8_plan(ids, weights, R, E, offsets, inv, f32(l.rw), ctx->err, st), "plan");
-    if (s != MPP41_OK) return s;
-    s = cuda_status(launch_fp8_scatter(d->fmt, x, T, H, inv, k, b + l.pq, f32(l.ps), Is ? b + l.xq : nullptr,
-                                       Is ? f32(l.xs) : nullptr, st), "quantize x");
+    s = cuda_status(launch_fp8_scatter(d->fmt, ids, weights, E, offsets, inv, f32(l.rw), ctx->err, x, T, H, k, b + l.pq, f32(l.ps),
+                                       Is ? b + l.xq : nullptr, Is ? f32(l.xs) : nullptr, st), "plan and quantize x");
     if (s != MPP41_OK) return s;
     Fp8Launch g{}, gs{}, n{}, ns{};
     g.a = b + l.pq; g.sa = f32(l.ps);

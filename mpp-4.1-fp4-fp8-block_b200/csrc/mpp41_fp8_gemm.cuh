@@ -667,10 +667,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 // mid = silu(gate) * up in fp32; one scale per row over the tile's 128
                 // channels, which this thread shares with the other column half's
                 float vmax = 0.0f;
+                if (live) {
 #pragma unroll
-                for (uint32_t i = 0; i < 64; ++i) {
-                    acc[i] = __fdividef(acc[i], 1.0f + __expf(-acc[i])) * acc[64 + i];
-                    vmax = fmaxf(vmax, fabsf(acc[i]));
+                    for (uint32_t i = 0; i < 64; ++i) {
+                        acc[i] = __fdividef(acc[i], 1.0f + __expf(-acc[i])) * acc[64 + i];
+                        vmax = fmaxf(vmax, fabsf(acc[i]));
+                    }
                 }
                 const uint32_t r = quarter * 32 + lane;
                 amax_x[half * 128 + r] = vmax;
@@ -678,22 +680,24 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 if (!alive) break;
                 vmax = fmaxf(amax_x[r], amax_x[128 + r]);
                 asm volatile("barrier.sync 1, %0;" ::"n"(kPromoThreads) : "memory");   // before the next tile's write
-                // below 1e-30 the group is zero for every output type; the floor keeps qmax / vmax finite
-                vmax = fminf(fmaxf(vmax, 1.0e-30f), 3.0e38f);
-                const float qmax = f8_max(p.out_fmt);
-                const float inv = __fdiv_rn(qmax, vmax);
+                if (live) {
+                    // below 1e-30 the group is zero for every output type; the floor keeps qmax / vmax finite
+                    vmax = fminf(fmaxf(vmax, 1.0e-30f), 3.0e38f);
+                    const float qmax = f8_max(p.out_fmt);
+                    const float inv = __fdiv_rn(qmax, vmax);
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    uint32_t w[4];
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        uint32_t w[4];
 #pragma unroll
-                    for (uint32_t q = 0; q < 4; ++q) {
-                        const float *v = acc + 16 * i + 4 * q;
-                        w[q] = enc_f8x2(p.out_fmt, v[0] * inv, v[1] * inv) | enc_f8x2(p.out_fmt, v[2] * inv, v[3] * inv) << 16;
+                        for (uint32_t q = 0; q < 4; ++q) {
+                            const float *v = acc + 16 * i + 4 * q;
+                            w[q] = enc_f8x2(p.out_fmt, v[0] * inv, v[1] * inv) | enc_f8x2(p.out_fmt, v[2] * inv, v[3] * inv) << 16;
+                        }
+                        stage_put(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
                     }
-                    stage_put(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
+                    stage_out(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
+                    if (row_ok && half == 0) sd.out_scales[(size_t)m * sd.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
                 }
-                stage_out(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
-                if (row_ok && half == 0) sd.out_scales[(size_t)m * sd.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
             } else if (live) {
                 if (sd.row_scale) {
                     const float f = row_ok ? sd.row_scale[m] : 0.0f;

@@ -157,9 +157,8 @@ cudaError_t launch_quantize_weights_fp8(int fmt, const float *w, uint32_t N, uin
 
 // Pieces of the FP8 expert layer (mpp41_moe_fp8.cu): n = T * k assignments; H % 128 == 0,
 // x 32-byte aligned; xq / xs (the unscattered rows) may be null.
-cudaError_t launch_fp8_plan(const int32_t *ids, const float *weights, uint32_t n, uint32_t E, int32_t *offsets,
-                            int32_t *inv, float *row_weight, uint32_t *err, cudaStream_t st);
-cudaError_t launch_fp8_scatter(int fmt, const void *x, uint32_t T, uint32_t H, const int32_t *inv, uint32_t k, uint8_t *pq,
+cudaError_t launch_fp8_scatter(int fmt, const int32_t *ids, const float *weights, uint32_t E, int32_t *offsets, int32_t *inv,
+                               float *row_weight, uint32_t *err, const void *x, uint32_t T, uint32_t H, uint32_t k, uint8_t *pq,
                                float *ps, uint8_t *xq, float *xs, cudaStream_t st);
 cudaError_t launch_fp8_combine(const void *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const void *shared_y,
                                void *out, int f16, cudaStream_t st);

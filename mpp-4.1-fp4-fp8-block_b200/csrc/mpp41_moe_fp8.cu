@@ -26,17 +26,17 @@ namespace fp8 {
 
 constexpr int kPlanThreads = 512;
 
-// One CTA an expert, each reading all ids twice (they sit in L2): rows before this
-// expert's = ids below it, then a stable compaction. Threads own contiguous runs
-// of assignments, so one block scan orders them. No launch or wait joins the CTAs.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__restrict__ ids, const float *__restrict__ weights,
-                                                            uint32_t n, uint32_t E, int32_t *__restrict__ offsets,
-                                                            int32_t *__restrict__ inv, float *__restrict__ row_weight, uint32_t *err)
+// Rows of expert e: one CTA reading all ids twice (they sit in L2): rows before e's = ids
+// below it, then a stable compaction. Threads own contiguous runs of assignments, so one
+// block scan orders them. No launch or wait joins the experts' CTAs.
+template <int THREADS>
+__device__ __forceinline__ void plan_expert(const int32_t *__restrict__ ids, const float *__restrict__ weights, uint32_t n, uint32_t E,
+                                            int32_t e, int32_t *__restrict__ offsets, int32_t *__restrict__ inv,
+                                            float *__restrict__ row_weight, uint32_t *err)
 {
-    __shared__ uint32_t sh_lt[kPlanThreads / 32], sh_eq[kPlanThreads / 32];
-    const int32_t e = (int32_t)blockIdx.x;
+    __shared__ uint32_t sh_lt[THREADS / 32], sh_eq[THREADS / 32];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t per = (n + kPlanThreads - 1) / kPlanThreads;
+    const uint32_t per = (n + THREADS - 1) / THREADS;
     const uint32_t a0 = min(threadIdx.x * per, n), a1 = min(a0 + per, n);
     uint32_t lt = 0, eq = 0;
     bool bad = false;
@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__res
     }
     __syncthreads();
     uint32_t base = 0, all = 0, before = 0;
-    for (uint32_t w = 0; w < kPlanThreads / 32; ++w) {
+#pragma unroll
+    for (uint32_t w = 0; w < THREADS / 32; ++w) {
         base += sh_lt[w];
         all += sh_eq[w];
         before += w < warp ? sh_eq[w] : 0u;
@@ -79,6 +80,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__res
                 row_weight[row] = weights[a];
                 inv[a] = (int32_t)row++;
             }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__restrict__ ids, const float *__restrict__ weights,
+                                                            uint32_t n, uint32_t E, int32_t *__restrict__ offsets,
+                                                            int32_t *__restrict__ inv, float *__restrict__ row_weight, uint32_t *err)
+{
+    plan_expert<kPlanThreads>(ids, weights, n, E, (int32_t)blockIdx.x, offsets, inv, row_weight, err);
 }
 
 // As the activation quantizer (8 lanes a block of 128, 16 values a lane), each block
@@ -116,14 +124,80 @@ __global__ void __launch_bounds__(256) quant_scatter_kernel(const uint8_t *__res
     }
 }
 
-// One CTA per (token, 2048 or 1024 columns): 16 bytes a thread; slots summed in order, fp32.
+// Plan and scatter in one launch, for few assignments: the first E CTAs plan, the others
+// scatter 32 blocks each and count the rows of their tokens' assignments themselves (ids
+// below theirs, and equal ones before theirs: a warp an assignment over all n ids).
+constexpr uint32_t kFewIds = 2048;       // ids kept in shared memory
+constexpr uint32_t kFewRows = 256;       // assignments a CTA counts for
+
+template <int FMT>
+__global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t *__restrict__ ids, const float *__restrict__ weights,
+                                                           uint32_t n, uint32_t E, int32_t *__restrict__ offsets,
+                                                           int32_t *__restrict__ inv, float *__restrict__ row_weight, uint32_t *err,
+                                                           const uint8_t *__restrict__ x, uint32_t kb, uint32_t blocks, uint32_t k,
+                                                           uint8_t *__restrict__ pq, float *__restrict__ ps,
+                                                           uint8_t *__restrict__ xq, float *__restrict__ xs)
+{
+    __shared__ int32_t sh_ids[kFewIds];
+    __shared__ int32_t rows[kFewRows];
+    if (blockIdx.x < E) {
+        plan_expert<256>(ids, weights, n, E, (int32_t)blockIdx.x, offsets, inv, row_weight, err);
+        return;
+    }
+    const uint32_t i0 = (blockIdx.x - E) * 32, i = i0 + threadIdx.x / 8, sub = threadIdx.x & 7;
+    const bool have = i < blocks;
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = 0u;
+    if (have) load_act16(x + ((size_t)i * 128 + sub * 16) * 2, w);
+    for (uint32_t a = threadIdx.x; a < n; a += 256) sh_ids[a] = ids[a];
+    __syncthreads();
+    const uint32_t t0 = i0 / kb, t1 = min(i0 + 31, blocks - 1) / kb, first = t0 * k, count = (t1 - t0 + 1) * k;
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t q = threadIdx.x >> 5; q < count; q += 8) {
+        const int32_t e = sh_ids[first + q];
+        uint32_t c = 0;
+        for (uint32_t a = lane; a < n; a += 32) {
+            const int32_t id = sh_ids[a];
+            c += id >= 0 && (id < e || (id == e && a < first + q)) ? 1u : 0u;
+        }
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (lane == 0) rows[q] = e >= 0 && e < (int32_t)E ? (int32_t)c : -1;
+    }
+    __syncthreads();
+    float scale;
+    const uint4 o = quant_act16<FMT>(w, scale);
+    if (!have) return;
+    const uint32_t t = i / kb, b = i - t * kb;
+    if (xq) {
+        *reinterpret_cast<uint4 *>(xq + (size_t)i * 128 + sub * 16) = o;
+        if (sub == 0) xs[i] = scale;
+    }
+    for (uint32_t j = 0; j < k; ++j) {
+        const int32_t r = rows[(t - t0) * k + j];
+        if (r < 0) continue;
+        const size_t at = (size_t)r * kb + b;
+        *reinterpret_cast<uint4 *>(pq + at * 128 + sub * 16) = o;
+        if (sub == 0) ps[at] = scale;
+    }
+}
+
+// One CTA per token and 128 units of 16 bytes; slots summed in order, fp32. A thread has
+// eight rows' loads in flight: with one token that is the whole kernel.
+constexpr int kCombineThreads = 128;
+
 template <bool F16>
-__global__ void __launch_bounds__(256) combine_fp8_kernel(const uint4 *__restrict__ y, const int32_t *__restrict__ inv,
-                                                          uint32_t k, uint32_t row16, const uint4 *__restrict__ shared_y,
-                                                          uint4 *__restrict__ out)
+__global__ void __launch_bounds__(kCombineThreads) combine_fp8_kernel(const uint4 *__restrict__ y, const int32_t *__restrict__ inv,
+                                                                      uint32_t k, uint32_t row16,
+                                                                      const uint4 *__restrict__ shared_y, uint4 *__restrict__ out)
 {
     constexpr int V = F16 ? 8 : 4;
-    const uint32_t t = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
+    __shared__ int32_t rows[32];
+    const uint32_t t = blockIdx.x, c = blockIdx.y * kCombineThreads + threadIdx.x;
+    if (threadIdx.x < k) rows[threadIdx.x] = inv[(size_t)t * k + threadIdx.x];
+    uint4 sh = make_uint4(0, 0, 0, 0);
+    if (shared_y && c < row16) sh = __ldcs(shared_y + (size_t)t * row16 + c);
+    __syncthreads();
     if (c >= row16) return;
     float acc[V];
 #pragma unroll
@@ -141,11 +215,16 @@ __global__ void __launch_bounds__(256) combine_fp8_kernel(const uint4 *__restric
             }
         }
     };
-    if (shared_y) add(__ldcs(shared_y + (size_t)t * row16 + c));
-#pragma unroll 4
-    for (uint32_t j = 0; j < k; ++j) {
-        const int32_t r = inv[(size_t)t * k + j];
-        if (r >= 0) add(__ldcs(y + (size_t)r * row16 + c));
+    add(sh);
+    for (uint32_t j0 = 0; j0 < k; j0 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            const int32_t r = j0 + j < k ? rows[j0 + j] : -1;
+            v[j] = r >= 0 ? __ldcs(y + (size_t)r * row16 + c) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) add(v[j]);
     }
     uint4 o;
     if (F16)
@@ -157,21 +236,30 @@ __global__ void __launch_bounds__(256) combine_fp8_kernel(const uint4 *__restric
 
 }  // namespace fp8
 
-cudaError_t launch_fp8_plan(const int32_t *ids, const float *weights, uint32_t n, uint32_t E, int32_t *offsets,
-                            int32_t *inv, float *row_weight, uint32_t *err, cudaStream_t st)
-{
-    fp8::plan_kernel<<<E, fp8::kPlanThreads, 0, st>>>(ids, weights, n, E, offsets, inv, row_weight, err);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_fp8_scatter(int fmt, const void *x, uint32_t T, uint32_t H, const int32_t *inv, uint32_t k, uint8_t *pq,
+cudaError_t launch_fp8_scatter(int fmt, const int32_t *ids, const float *weights, uint32_t E, int32_t *offsets, int32_t *inv,
+                               float *row_weight, uint32_t *err, const void *x, uint32_t T, uint32_t H, uint32_t k, uint8_t *pq,
                                float *ps, uint8_t *xq, float *xs, cudaStream_t st)
 {
-    const uint64_t blocks = (uint64_t)T * (H / 128), need = (blocks + 31) / 32;
-    const unsigned grid = (unsigned)(need < 148 * 16 ? need : 148 * 16);
+    using namespace fp8;
+    const uint32_t n = T * k, kb = H / 128;
+    const uint64_t blocks = (uint64_t)T * kb, need = (blocks + 31) / 32;
     const uint8_t *xb = static_cast<const uint8_t *>(x);
-    if (fmt == 1) fp8::quant_scatter_kernel<1><<<grid, 256, 0, st>>>(xb, H / 128, blocks, inv, k, pq, ps, xq, xs);
-    else fp8::quant_scatter_kernel<2><<<grid, 256, 0, st>>>(xb, H / 128, blocks, inv, k, pq, ps, xq, xs);
+    // one launch (3 us less) where counting stays short: a CTA's assignments times all ids
+    const uint64_t mine = (31 / kb + 2) * (uint64_t)k;
+    if (n <= kFewIds && mine <= kFewRows && mine * n <= 32768) {
+        const unsigned grid = E + (unsigned)need;
+        if (fmt == 1)
+            plan_scatter_kernel<1><<<grid, 256, 0, st>>>(ids, weights, n, E, offsets, inv, row_weight, err, xb, kb, (uint32_t)blocks, k, pq, ps, xq, xs);
+        else
+            plan_scatter_kernel<2><<<grid, 256, 0, st>>>(ids, weights, n, E, offsets, inv, row_weight, err, xb, kb, (uint32_t)blocks, k, pq, ps, xq, xs);
+        return cudaGetLastError();
+    }
+    plan_kernel<<<E, kPlanThreads, 0, st>>>(ids, weights, n, E, offsets, inv, row_weight, err);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const unsigned grid = (unsigned)(need < 148 * 16 ? need : 148 * 16);
+    if (fmt == 1) quant_scatter_kernel<1><<<grid, 256, 0, st>>>(xb, kb, blocks, inv, k, pq, ps, xq, xs);
+    else quant_scatter_kernel<2><<<grid, 256, 0, st>>>(xb, kb, blocks, inv, k, pq, ps, xq, xs);
     return cudaGetLastError();
 }
 
@@ -179,10 +267,10 @@ cudaError_t launch_fp8_combine(const void *y, const int32_t *inv, uint32_t T, ui
                                void *out, int f16, cudaStream_t st)
 {
     const uint32_t row16 = H / (f16 ? 8 : 4);
-    const dim3 grid(T, (row16 + 255) / 256);
+    const dim3 grid(T, (row16 + fp8::kCombineThreads - 1) / fp8::kCombineThreads);
     const uint4 *a = static_cast<const uint4 *>(y), *sy = static_cast<const uint4 *>(shared_y);
-    if (f16) fp8::combine_fp8_kernel<true><<<grid, 256, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
-    else fp8::combine_fp8_kernel<false><<<grid, 256, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
+    if (f16) fp8::combine_fp8_kernel<true><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
+    else fp8::combine_fp8_kernel<false><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
     return cudaGetLastError();
 }
 
