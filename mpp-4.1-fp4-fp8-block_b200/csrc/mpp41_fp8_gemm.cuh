@@ -603,45 +603,42 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 }
             };
             if (live) {
-                // Scales a block ahead, in registers that the unrolled loop names in turn:
-                // moving them on would wait for the loads.
-                float a[2], u0[2], u1[2];
-                auto fetch = [&](uint32_t kk, uint32_t i) {
+                // Scales a block ahead: taken over at the top of the next block, when their loads
+                // have had a whole block's time. One body, not unrolled: its code, the MMA
+                // issuer's and the producers' share the instruction cache.
+                float an = 0.0f, u0n = 0.0f, u1n = 0.0f;
+                auto fetch = [&](uint32_t kk) {
                     if (kk < k1) {
-                        a[i] = __ldg(sa + kk);
-                        u0[i] = __ldg(sb0 + kk);
-                        if constexpr (kRuns == 2) u1[i] = __ldg(sb1 + kk);
+                        an = __ldg(sa + kk);
+                        u0n = __ldg(sb0 + kk);
+                        if constexpr (kRuns == 2) u1n = __ldg(sb1 + kk);
                     }
                 };
-                fetch(k0, 0);
-                for (uint32_t kq = k0; kq < k1 && alive; kq += 2) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 2; ++i) {
-                        if (kq + i >= k1) break;
-                        fetch(kq + i + 1, i ^ 1u);
-                        const uint32_t b = g % NA;
-                        if (!wait_all(&acc_full[b], (g / NA) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
-                        ++g;
-                        tc_fence_after();
-                        const uint32_t base = tmem + lane_base + b * BN + half * 64;
-                        const float s0 = a[i] * u0[i], s1 = kRuns == 2 ? a[i] * u1[i] : s0;
-                        uint32_t d[32], e[32];
-                        tmem_ld_32x32b_x32(base, d);
-                        tmem_ld_32x32b_x32(base + 32, e);
+                fetch(k0);
+#pragma unroll 1
+                for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
+                    const float s0 = an * u0n, s1 = kRuns == 2 ? an * u1n : s0;
+                    fetch(kk + 1);
+                    const uint32_t b = g % NA;
+                    if (!wait_all(&acc_full[b], (g / NA) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
+                    tc_fence_after();
+                    const uint32_t base = tmem + lane_base + b * BN + half * 64;
+                    uint32_t d[32], e[32];
+                    tmem_ld_32x32b_x32(base, d);
+                    tmem_ld_32x32b_x32(base + 32, e);
+                    tmem_ld_wait32(d);
+                    tmem_ld_wait32(e);
+                    if constexpr (kRuns == 2) {
+                        promote32(acc, d, s0);
+                        promote32(acc + 32, e, s0);
+                        tmem_ld_32x32b_x32(base + 128, d);
+                        tmem_ld_32x32b_x32(base + 160, e);
                         tmem_ld_wait32(d);
                         tmem_ld_wait32(e);
-                        if constexpr (kRuns == 2) {
-                            promote32(acc, d, s0);
-                            promote32(acc + 32, e, s0);
-                            tmem_ld_32x32b_x32(base + 128, d);
-                            tmem_ld_32x32b_x32(base + 160, e);
-                            tmem_ld_wait32(d);
-                            tmem_ld_wait32(e);
-                        }
-                        release(b);
-                        promote32(acc + kRuns * 64 - 64, d, s1);
-                        promote32(acc + kRuns * 64 - 32, e, s1);
                     }
+                    release(b);
+                    promote32(acc + kRuns * 64 - 64, d, s1);
+                    promote32(acc + kRuns * 64 - 32, e, s1);
                 }
             } else {
                 for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
