@@ -125,3 +125,27 @@ def test_tiny_scores_keep_their_ratio(ctx, z0):
     z = (z0 + np.arange(16, dtype=np.float32))[None].repeat(2, 0)
     for sigmoid in (True, False):
         check(ctx, z, None, 4, sigmoid=sigmoid)
+
+
+@pytest.mark.parametrize("sigmoid", [True, False])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("e,k,groups,top_groups,group_top", [
+    (64, 6, 1, 1, 1), (64, 8, 4, 2, 2), (40, 5, 5, 3, 1), (7, 3, 1, 1, 1), (129, 9, 1, 1, 1),
+])
+def test_many_tokens(ctx, e, k, groups, top_groups, group_top, sigmoid, renorm):
+    """From the token counts of a long prefill on, a warp weighs several tokens' choices
+    together: a ragged last batch, ties, masks and near ties among its tokens."""
+    t = 148 * 64 + 7
+    rng = np.random.default_rng(e)
+    z = (rng.standard_normal((t, e)) * 2).astype(np.float32)
+    z[5] = 0.0
+    z[6] = -np.inf
+    z[7] = np.nan
+    z[8, 1:] = -np.inf
+    z[9] = 18.0 + rng.permutation(e) * 1e-3
+    z[10] = rng.permutation(e) * 1e-7
+    z[-1] = np.inf
+    kw = dict(sigmoid=sigmoid, groups=groups, top_groups=top_groups, group_top=group_top, renorm=renorm, scale=2.5)
+    check(ctx, z, (0.2 * rng.standard_normal(e)).astype(np.float32), k, **kw)
+    check(ctx, z, None, k, **kw)
+    check(ctx, z.astype(np.float16), None, k, **kw)
