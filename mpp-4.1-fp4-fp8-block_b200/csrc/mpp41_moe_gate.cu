@@ -6,9 +6,9 @@
 // largest v; the top_groups best groups stay, and the top_k experts are taken
 // from them by falling v, ties to the lower index.
 //
-// The selection is exact: it is the one the 64-bit values give. Without a bias
-// (and without sums of two scores) v is monotone in the logit, so the logits are
-// compared themselves. Otherwise fp32 scores decide, and wherever two values that
+// The selection is exact: it is the one the 64-bit values give. Without a bias v is
+// monotone in the logit, so experts (and groups by their best expert) are compared by
+// the logits themselves. Otherwise fp32 scores decide, and wherever two values that
 // the outcome depends on lie closer than the fp32 error, that warp decides the
 // token again in 64 bits (exact_token, about 3 us): a few tokens in a thousand for
 // scores of a trained router's spread.
@@ -18,8 +18,7 @@
 // then one warp-wide maximum of the lanes' heads and a shift in the winner's lane.
 // A group is a run of lanes, its two best a butterfly. 32768 tokens of 256 experts are
 // bound by instruction issue, not by the 34 MB they read.
-// any_kernel (every token through exact_token) takes the group sizes that do not fall
-// on lane borders.
+// Groups that do not fall on lane borders go through shared memory.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -40,7 +39,9 @@ struct Params {
     int32_t *ids;           // [T][k]
     float *weights;         // [T][k]
     uint32_t T, E, k, groups, top_groups, group_top, group_size;
-    int sigmoid, renorm, f16, by_logit;   // by_logit: v is the logit
+    int sigmoid, renorm, f16;
+    int by_logit;                         // experts are compared by their logits (no bias)
+    int scores;                           // scores are needed: a bias, or sums of two for the groups
     int vec;                              // rows of logits start on 16 bytes
     float scale;
 };
@@ -93,7 +94,7 @@ __device__ __noinline__ uint32_t exact_token(const Params &p, size_t row, uint32
     double v[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) v[j] = lane + 32 * j < p.E ? (double)load_logit(p, row + lane + 32 * j) : -inf;
-    if (!p.by_logit) {
+    if (p.scores) {
         uint32_t masked = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) masked |= v[j] > -inf ? 0u : 1u << j;
@@ -163,6 +164,7 @@ __device__ __noinline__ uint32_t exact_token(const Params &p, size_t row, uint32
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const uint32_t e = lane + 32 * j;
+        if (p.by_logit && p.scores && e < p.E) v[j] = (double)load_logit(p, row + e);
         key[j] = e < p.E && (keep == kFull || keep >> (e / p.group_size) & 1u) ? order_bits64(v[j] + 0.0) : 0ull;
     }
     uint32_t mine = 0;
@@ -233,30 +235,6 @@ template <int PER> __device__ __forceinline__ void softmax_norm(const float (&z)
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
 }
 
-template <int PER>
-__global__ void __launch_bounds__(32 * kWarps) any_kernel(const Params p)
-{
-    extern __shared__ double smem[];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t t = blockIdx.x * kWarps + warp;
-    pdl_launch_dependents();
-    pdl_wait_prior();
-    if (t >= p.T) return;
-    const size_t row = (size_t)t * p.E;
-    const uint32_t e = exact_token<PER>(p, row, lane, smem + (size_t)warp * p.E);
-    float m = -INFINITY, sum = 0.0f;
-    if (!p.renorm && !p.sigmoid) {
-        for (uint32_t i = lane; i < p.E; i += 32) m = fmaxf(m, load_logit(p, row + i));
-        m = warp_max(m);
-        for (uint32_t i = lane; i < p.E; i += 32) {
-            const float z = load_logit(p, row + i);
-            sum += z > -INFINITY ? (z == m ? 1.0f : expf(z - m)) : 0.0f;
-        }
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-    }
-    write_slot(p, t, lane, 32, true, e, m, sum);
-}
-
 // Order-preserving bits of a float (not NaN); never 0.
 __device__ __forceinline__ uint32_t order_bits(float v)
 {
@@ -320,11 +298,12 @@ __device__ __forceinline__ void load_lane(const Params &p, uint32_t t, uint32_t 
     }
 }
 
-// group_lanes: lanes a group takes (a power of two) where groups are dropped, else 0.
+// lanes: where groups are dropped, the lanes a group takes (a power of two): its experts
+// lie in them, or (SMEM_GROUPS) they read them from shared memory; else 0.
 // A warp chooses for `batch` tokens, one after the other, and then weighs their choices
 // together, kp lanes a token (batch * kp <= 32).
-template <int PER, bool F16>
-__global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(const Params p, uint32_t group_lanes, uint32_t batch, uint32_t kp)
+template <int PER, bool F16, bool SMEM_GROUPS>
+__global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(const Params p, uint32_t lanes, uint32_t batch, uint32_t kp)
 {
     extern __shared__ double smem[];
     __shared__ uint32_t sel[kWarps][32];
@@ -350,9 +329,10 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
     // 2^-21 (and 2^-23 |v| for larger ones). A softmax's sum is off by one factor for all,
     // at most PER + 10 half ulps. Logits compared themselves have no error. Keys cut to
     // their upper bits keep the order; equal ones are less than one cut unit apart.
-    const float tol = p.by_logit ? 0.0f : (p.sigmoid ? 0.0f : (float)(PER + 10) / 16777216.0f) + 1.0f / 2097152.0f;
+    const float err = (p.sigmoid ? 0.0f : (float)(PER + 10) / 16777216.0f) + 1.0f / 2097152.0f, tol = p.by_logit ? 0.0f : err;
     const float unit = ((float)(1u << kBits) + (p.by_logit ? 0.0f : 1.0f)) / 8388608.0f;
-    const bool ragged = p.E % PER != 0;
+    const bool ragged = p.E % PER != 0 || lane * PER >= p.E;
+    const float inv_size = __fdividef(1.0f, (float)p.group_size);
     const bool check = !(p.by_logit && F16);   // fp16 logits lose no bits to the position
     for (uint64_t t0 = (uint64_t)(blockIdx.x * kWarps + warp) * batch; t0 < p.T; t0 += stride) {
         const uint32_t n = (uint32_t)min((uint64_t)batch, p.T - t0);
@@ -360,7 +340,7 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
             const uint32_t t = (uint32_t)t0 + i;
             float z[PER], v[PER];
             load_lane<PER, F16>(p, t, lane, z);
-            if (p.by_logit) {
+            if (!p.scores) {
 #pragma unroll
                 for (int j = 0; j < PER; ++j) v[j] = z[j] > -INFINITY ? z[j] + 0.0f : -INFINITY;   // NaN masks; -0 -> +0
             } else if (p.sigmoid) {
@@ -390,46 +370,79 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
                     if (!(z[j] > -INFINITY)) v[j] = -INFINITY;
                 }
             }
-            bool sure = true, keep = lane * PER < p.E;
-            if (group_lanes) {
-                float b0 = v[0], b1 = -INFINITY;
+            bool sure = true;
+            uint32_t stay = kFull;   // bit g: group g stays
+            if (lanes) {
+                float b0 = -INFINITY, b1 = -INFINITY;
+                const uint32_t mine = lane / lanes;
+                if constexpr (!SMEM_GROUPS) {
 #pragma unroll
-                for (int j = 1; j < PER; ++j) {
-                    b1 = fmaxf(b1, fminf(b0, v[j]));
-                    b0 = fmaxf(b0, v[j]);
+                    for (int j = 0; j < PER; ++j) {
+                        b1 = fmaxf(b1, fminf(b0, v[j]));
+                        b0 = fmaxf(b0, v[j]);
+                    }
+                } else {
+                    float *sf = reinterpret_cast<float *>(sv);
+#pragma unroll
+                    for (int j = 0; j < PER; ++j)
+                        if (lane * PER + j < p.E) sf[lane * PER + j] = v[j];
+                    __syncwarp();
+                    if (mine < p.groups)
+                        for (uint32_t q = lane % lanes; q < p.group_size; q += lanes) {
+                            const float x = sf[mine * p.group_size + q];
+                            b1 = fmaxf(b1, fminf(b0, x));
+                            b0 = fmaxf(b0, x);
+                        }
+                    __syncwarp();
                 }
-                for (uint32_t o = group_lanes >> 1; o; o >>= 1) {
+                for (uint32_t o = lanes >> 1; o; o >>= 1) {
                     const float o0 = __shfl_xor_sync(kFull, b0, o), o1 = __shfl_xor_sync(kFull, b1, o);
                     b1 = fmaxf(fminf(b0, o0), fmaxf(b1, o1));
                     b0 = fmaxf(b0, o0);
                 }
                 const float worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
-                const uint32_t mine = lane / group_lanes;
                 uint32_t rank = 0;
-                if (p.by_logit) {
+                if (!p.scores) {
                     for (uint32_t g = 0; g < p.groups; ++g) {
-                        const float w = __shfl_sync(kFull, worth, g * group_lanes);
+                        const float w = __shfl_sync(kFull, worth, g * lanes);
                         rank += w > worth || (w == worth && g < mine) ? 1u : 0u;
                     }
-                } else {   // a tie at the cut is not sure anyway
+                } else {   // groups tied at the cut all stay: too many, which is not sure
 #pragma unroll 4
                     for (uint32_t g = 0; g < p.groups; ++g)
-                        rank += __shfl_sync(kFull, worth, g * group_lanes) > worth ? 1u : 0u;
+                        rank += __shfl_sync(kFull, worth, g * lanes) > worth ? 1u : 0u;
                 }
                 const bool real = mine < p.groups;
-                keep = real && rank < p.top_groups;
-                if (!p.by_logit) {
+                const bool keep = real && rank < p.top_groups;
+                const uint32_t in_lanes = __ballot_sync(kFull, keep);
+                if constexpr (!SMEM_GROUPS) {
+                    stay = keep ? kFull : 0u;   // of this lane's group
+                } else {
+                    stay = 0u;
+                    for (uint32_t g = 0; g < p.groups; ++g) stay |= (in_lanes >> (g * lanes) & 1u) << g;
+                }
+                if (p.scores) {
                     // the last group that stays and the first that goes have to be well apart
                     const uint32_t k = order_bits(worth);
                     const float in = order_value(__reduce_min_sync(kFull, keep ? k : 0xFFFFFFFFu));
                     const float out = order_value(__reduce_max_sync(kFull, real && !keep ? k : 0u));
-                    sure = in - out > 2.0f * tol + fabsf(in) * (1.0f / 4194304.0f);   // sums of two
+                    sure = __popc(in_lanes) == p.top_groups * lanes &&
+                           in - out > 2.0f * err + fabsf(in) * (1.0f / 4194304.0f);   // sums of two
                 }
             }
             uint32_t key[PER];
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                key[j] = keep ? (order_bits(v[j]) & ~kLow) | (kLow - (uint32_t)j) : 0u;
+                float x = v[j];
+                if (p.by_logit && p.scores) x = z[j] > -INFINITY ? z[j] + 0.0f : -INFINITY;
+                key[j] = (order_bits(x) & ~kLow) | (kLow - (uint32_t)j);
+                if constexpr (SMEM_GROUPS) {
+                    // e / group_size by the reciprocal: exact below 512
+                    const uint32_t g = (uint32_t)(((float)(lane * PER + j) + 0.5f) * inv_size);
+                    if (!(stay >> (g & 31u) & 1u)) key[j] = 0u;
+                } else if (!stay) {
+                    key[j] = 0u;
+                }
                 if (ragged && lane * PER + j >= p.E) key[j] = 0u;
             }
             sort_desc<PER>(key);
@@ -462,6 +475,8 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
                     const float a = order_value(won & ~kLow), b = order_value(next & ~kLow);
                     sure = sure && (won >> kBits) != (next >> kBits) && a - b > tol + fmaxf(fabsf(a), fabsf(b)) * unit * (p.by_logit ? 0.0f : 1.0f);
                 }
+            }
+            if (check || p.scores) {
                 if (!__all_sync(kFull, sure)) {
                     __syncwarp();
                     const uint32_t e = exact_token<kExactPer>(p, (size_t)t * p.E, lane, sv);
@@ -485,7 +500,7 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
     }
 }
 
-template <bool F16> cudaError_t launch_fast(const Params &p, uint32_t per, uint32_t group_lanes, cudaStream_t st)
+template <bool F16, bool SMEM_GROUPS> cudaError_t launch_fast(const Params &p, uint32_t per, uint32_t lanes, cudaStream_t st)
 {
     // Weighing a token's k choices leaves most lanes idle: from enough tokens for every
     // warp slot, a warp weighs as many together as fit its lanes.
@@ -494,9 +509,9 @@ template <bool F16> cudaError_t launch_fast(const Params &p, uint32_t per, uint3
     const uint32_t most = 148 * 7, batch = p.T >= most * kWarps ? 32 / kp : 1;
     const uint64_t per_cta = (uint64_t)kWarps * batch, want = (p.T + per_cta - 1) / per_cta;
     const unsigned grid = (unsigned)(want < most ? want : most);
-    const size_t smem = group_lanes ? (size_t)kWarps * p.E * sizeof(double) : 0;
+    const size_t smem = lanes ? (size_t)kWarps * p.E * sizeof(double) : 0;
     switch (per) {
-#define GATE_CASE(N) case N: return launch_overlapped(fast_kernel<N, F16>, dim3(grid), dim3(32 * kWarps), smem, st, p, group_lanes, batch, kp);
+#define GATE_CASE(N) case N: return launch_overlapped(fast_kernel<N, F16, SMEM_GROUPS>, dim3(grid), dim3(32 * kWarps), smem, st, p, lanes, batch, kp);
     GATE_CASE(1) GATE_CASE(2) GATE_CASE(3) GATE_CASE(4) GATE_CASE(5) GATE_CASE(6) GATE_CASE(8) GATE_CASE(10) GATE_CASE(12)
     GATE_CASE(16)
 #undef GATE_CASE
@@ -515,23 +530,28 @@ cudaError_t launch_moe_gate(const GateLaunch &L, cudaStream_t st)
     p.T = L.T; p.E = L.E; p.k = L.k;
     p.groups = L.groups; p.top_groups = L.top_groups; p.group_top = L.group_top; p.group_size = L.E / L.groups;
     p.sigmoid = L.sigmoid; p.renorm = L.renorm; p.f16 = L.f16;
-    // one score's order is its logit's; only a bias or a sum of two needs the scores
-    p.by_logit = !L.bias && (L.top_groups == L.groups || L.group_top == 1 || p.group_size == 1);
+    p.by_logit = !L.bias;
+    p.scores = L.bias || (L.top_groups < L.groups && L.group_top == 2 && p.group_size > 1);
     p.scale = L.scale;
     p.vec = (size_t)L.E * (L.f16 ? 2 : 4) % 16 == 0 && (reinterpret_cast<uintptr_t>(L.logits) & 15u) == 0;
     const bool grouped = L.top_groups < L.groups;
-    // experts a lane: the fewest that hold all, and a group in a power of two of lanes
-    for (uint32_t per : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 10u, 12u, 16u}) {
-        if (per * 32 < L.E) continue;
-        if (!grouped) return L.f16 ? launch_fast<true>(p, per, 0, st) : launch_fast<false>(p, per, 0, st);
-        const uint32_t lanes = p.group_size / per;
-        if (p.group_size % per || (lanes & (lanes - 1))) continue;
-        return L.f16 ? launch_fast<true>(p, per, lanes, st) : launch_fast<false>(p, per, lanes, st);
+    // Experts a lane: the fewest that hold all; where groups are dropped rather up to twice
+    // that, if a group then lies in a power of two of lanes.
+    uint32_t per = 0, lanes = 0, least = 0;
+    for (uint32_t c : {1u, 2u, 3u, 4u, 5u, 6u, 8u, 10u, 12u, 16u}) {
+        if (c * 32 < L.E) continue;
+        if (!least) least = c;
+        const uint32_t in = p.group_size / c;
+        if (!grouped || (c <= 2 * least && p.group_size % c == 0 && !(in & (in - 1)))) {
+            per = c;
+            lanes = grouped ? in : 0;
+            break;
+        }
     }
-    const unsigned grid = (L.T + kWarps - 1) / kWarps;
-    const size_t smem = (size_t)kWarps * L.E * sizeof(double);
-    return launch_overlapped(L.E <= 64 ? any_kernel<2> : L.E <= 128 ? any_kernel<4> : L.E <= 256 ? any_kernel<8> : any_kernel<16>,
-                             dim3(grid), dim3(32 * kWarps), smem, st, p);
+    if (per) return L.f16 ? launch_fast<true, false>(p, per, lanes, st) : launch_fast<false, false>(p, per, lanes, st);
+    lanes = 32;
+    while (lanes * p.groups > 32 && lanes > 1) lanes >>= 1;
+    return L.f16 ? launch_fast<true, true>(p, least, lanes, st) : launch_fast<false, true>(p, least, lanes, st);
 }
 
 }  // namespace mpp41

@@ -73,18 +73,18 @@ def gate(z, bias, k, sigmoid, groups, top_groups, group_top, renorm, scale):
                 x = np.where(masked, 0.0, x)
                 s = x / x.sum() if x.sum() > 0 else x
             v = s + (0.0 if bias is None else np.asarray(bias, np.float64))
-        if bias is None and (top_groups == groups or min(group_top, size) == 1):
-            v = zr          # one score's order is its logit's, also where 64 bits saturate
         v = np.where(masked | np.isnan(v), -np.inf, v)
+        order = zr if bias is None else v   # without a bias by the logits, also where 64 bits saturate
         if groups > 1:
-            per = np.sort(v.reshape(groups, size), axis=1)[:, ::-1]
+            one = min(group_top, size) == 1
+            per = np.sort((order if one else v).reshape(groups, size), axis=1)[:, ::-1]
             worth = per[:, :min(group_top, size)].sum(axis=1)
             stay = np.argsort(-worth, kind="stable")[:top_groups]
             inside = np.isin(np.arange(e) // size, stay)
         else:
             inside = np.ones(e, bool)
         cand = np.nonzero(inside)[0]
-        pick = cand[np.argsort(-v[cand], kind="stable")[:k]]
+        pick = cand[np.argsort(-order[cand], kind="stable")[:k]]
         ids[r] = pick
         with np.errstate(over="ignore", invalid="ignore"):
             if renorm and not masked[pick].all():
