@@ -122,9 +122,10 @@ int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || dev >= kMaxDevices) { *why = "device"; return 2; }
     // Row tiles at most (a group's last may be partial), of 128 rows and of a pair's 256.
-    // Pairs from 1024 rows a group: 4 to 6 % faster there (4096 x 14336 x 4096: 248 against
-    // 258 us), but their 256-row tiles round groups up further (32 groups of 512 rows on
-    // average: 311 against 296 us; of 256: 708 against 632 us for the whole layer).
+    // Pairs from 1024 rows a group: 4 to 5 % faster there (4096 x 14336 x 4096: 229 against
+    // 238 us, 8192^3: 514 against 540), but their 256-row tiles round groups up further (32
+    // groups of 512 rows on average: 287 against 265 us; a layer with 128 rows an expert:
+    // 439 against 370).
     const uint64_t mt = L.offsets ? L.M / kBM + (L.groups < L.M ? L.groups : L.M) : (L.M + kBM - 1) / kBM;
     const uint64_t sms = (uint64_t)sm_count(dev);
     const bool few = !swiglu && !L.offsets && !more && mt * ((L.N + 255) / 256) < sms && mt * ((L.N + 127) / 128) <= sms;

@@ -18,10 +18,16 @@
 // are neither loaded nor promoted (32-row granularity).
 //
 // Warp roles (384 threads): 0 TMA producer of B, 1 MMA issuer and TMEM owner, 2 TMA
-// producer of A, 3 idle (it holds registers that the promotion warps take over), 4..11 promotion (warp w: TMEM lane
-// quarter w % 4, column half (w - 4) / 4). One warp for copies and MMAs ran the
-// 4096 x 14336 x 4096 product a third slower: a block's copies take it as long to issue
-// as the block's MMAs take to run.
+// producer of A, 3 the groups' tables (then its registers go to the promotion warps),
+// 4..11 promotion (warp w: TMEM lane quarter w % 4, column half (w - 4) / 4). With one
+// warp for copies and MMAs the 4096 x 14336 x 4096 product took 360 us: a block's copies
+// take it as long to issue as the block's MMAs take to run. Sixteen promotion warps of
+// half the columns (112 registers each) took 276 us.
+//
+// What bounds it: with many rows the promotion. That product takes 224 to 229 us
+// (2.1 PFLOP/s); of 244 us in an earlier form 48 went without the FMAs, 63 without reading
+// tensor memory either, 17 without the copies, and the epilogue's stores cost 20 of 230.
+// With few rows it is the stream of B from memory.
 #pragma once
 
 #include <cuda.h>
@@ -59,10 +65,13 @@ template <int BN, int AR, int MODE> struct Cfg {
     static constexpr uint32_t kTileRows = MODE == PAIR ? 256 : 128;
     static constexpr uint32_t kAStage = AR * kBK;
     static constexpr uint32_t kBStage = (MODE == PAIR ? 1 : kRuns) * kBTile;   // PAIR: run `rank` only
-    static constexpr int kStages = MODE == PAIR ? 6 : BN == 256 ? 4 : (AR == 32 ? 9 : 6);
+    static constexpr int kStages = MODE == PAIR ? 5 : BN == 256 ? 4 : (AR == 32 ? 9 : 6);
+    // 16-byte units of a staged output row. PAIR takes the sixth stage's room for 128-byte
+    // rows (4096 x 7168 x 2048, fp32 C: 77.7 against 81.3 us; one stage less costs nothing).
+    static constexpr uint32_t kUnits = MODE == PAIR ? 8 : 4;
     static constexpr uint32_t kOffB = ((kStages * kAStage + 1023) / 1024) * 1024;
-    static constexpr uint32_t kOffOut = kOffB + kStages * kBStage;  // 8 warps x 2 KB, epilogue transposition
-    static constexpr uint32_t kOffAmax = kOffOut + 8 * 2048;        // SwiGLU: [2 halves][128] floats
+    static constexpr uint32_t kOffOut = kOffB + kStages * kBStage;  // 32 rows a promotion warp, epilogue transposition
+    static constexpr uint32_t kOffAmax = kOffOut + 8 * 512 * kUnits;        // SwiGLU: [2 halves][128] floats
     static constexpr uint32_t kOffBar = kOffAmax + 1024;
     static constexpr uint32_t kOffGroups = kOffBar + 256;           // 3 words per group + 1
     static constexpr uint32_t kSmem = kOffGroups;                   // + group_bytes(all_groups)
@@ -208,24 +217,64 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Completion of this thread's tcgen05.ld, tied to the registers it fills so that no use moves above it.
-__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&r)[32])
+// 64 columns of this warp's lanes, complete, as pairs of neighbouring columns. Load, wait
+// and pairing are one statement: the pairs are then the loaded registers themselves.
+__device__ __forceinline__ void tmem_ld_pairs(uint32_t taddr, uint64_t (&r)[32])
 {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
+    asm volatile("{\n\t.reg .b32 t<64>;\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12, t13, t14, t15, t16, t17, t18, t19, t20, t21, t22, t23, t24, t25, t26, t27, t28, t29, t30, t31, t32, t33, t34, t35, t36, t37, t38, t39, t40, t41, t42, t43, t44, t45, t46, t47, t48, t49, t50, t51, t52, t53, t54, t55, t56, t57, t58, t59, t60, t61, t62, t63}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n\t"
+        "mov.b64 %0, {t0, t1};\n\t"
+        "mov.b64 %1, {t2, t3};\n\t"
+        "mov.b64 %2, {t4, t5};\n\t"
+        "mov.b64 %3, {t6, t7};\n\t"
+        "mov.b64 %4, {t8, t9};\n\t"
+        "mov.b64 %5, {t10, t11};\n\t"
+        "mov.b64 %6, {t12, t13};\n\t"
+        "mov.b64 %7, {t14, t15};\n\t"
+        "mov.b64 %8, {t16, t17};\n\t"
+        "mov.b64 %9, {t18, t19};\n\t"
+        "mov.b64 %10, {t20, t21};\n\t"
+        "mov.b64 %11, {t22, t23};\n\t"
+        "mov.b64 %12, {t24, t25};\n\t"
+        "mov.b64 %13, {t26, t27};\n\t"
+        "mov.b64 %14, {t28, t29};\n\t"
+        "mov.b64 %15, {t30, t31};\n\t"
+        "mov.b64 %16, {t32, t33};\n\t"
+        "mov.b64 %17, {t34, t35};\n\t"
+        "mov.b64 %18, {t36, t37};\n\t"
+        "mov.b64 %19, {t38, t39};\n\t"
+        "mov.b64 %20, {t40, t41};\n\t"
+        "mov.b64 %21, {t42, t43};\n\t"
+        "mov.b64 %22, {t44, t45};\n\t"
+        "mov.b64 %23, {t46, t47};\n\t"
+        "mov.b64 %24, {t48, t49};\n\t"
+        "mov.b64 %25, {t50, t51};\n\t"
+        "mov.b64 %26, {t52, t53};\n\t"
+        "mov.b64 %27, {t54, t55};\n\t"
+        "mov.b64 %28, {t56, t57};\n\t"
+        "mov.b64 %29, {t58, t59};\n\t"
+        "mov.b64 %30, {t60, t61};\n\t"
+        "mov.b64 %31, {t62, t63};\n\t"
+        "}"
+        : "=l"(r[0]), "=l"(r[1]), "=l"(r[2]), "=l"(r[3]), "=l"(r[4]), "=l"(r[5]), "=l"(r[6]), "=l"(r[7]), "=l"(r[8]), "=l"(r[9]), "=l"(r[10]), "=l"(r[11]), "=l"(r[12]), "=l"(r[13]), "=l"(r[14]), "=l"(r[15]), "=l"(r[16]), "=l"(r[17]), "=l"(r[18]), "=l"(r[19]), "=l"(r[20]), "=l"(r[21]), "=l"(r[22]), "=l"(r[23]), "=l"(r[24]), "=l"(r[25]), "=l"(r[26]), "=l"(r[27]), "=l"(r[28]), "=l"(r[29]), "=l"(r[30]), "=l"(r[31])
+        : "r"(taddr) : "memory");
 }
 
-// acc[i] += d[i] * s. Scalar FMAs: the packed fp32 form needs its operands moved into
-// register pairs, and ran the 4096 x 14336 x 4096 product at 400 us against 292 us.
-__device__ __forceinline__ void promote32(float *acc, const uint32_t (&d)[32], float s)
+// acc += d * s on pairs: half the instructions of scalar FMAs, which the promotion warps
+// share their schedulers and instruction cache with the MMA issuer and the producers for
+// (4096 x 14336 x 4096: 234 against 237 us, 32 groups of 512 rows: 273 against 280).
+__device__ __forceinline__ void promote_pairs(uint64_t *acc, const uint64_t (&d)[32], uint64_t s)
 {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = fmaf(__uint_as_float(d[i]), s, acc[i]);
+    for (int i = 0; i < 32; ++i) asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i]) : "l"(d[i]), "l"(s));
+}
+
+__device__ __forceinline__ uint64_t dup2(float s)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(s));
+    return r;
 }
 
 // Barrier of the promotion warps that also ORs a flag.
@@ -312,33 +361,35 @@ __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uin
     if (lane == 31) cum[p.all_groups] = inc;
 }
 
-// ---- epilogue: 32 rows x 64 bytes of a warp through shared memory (2 KB, 16-byte units
-// rotated by the row), so that a store instruction covers eight whole 64-byte row
-// segments instead of 32 rows' 16 bytes.
-__device__ __forceinline__ void stage_put(uint8_t *buf, uint32_t lane, uint32_t j, uint4 v)
+// ---- epilogue: 32 rows of U 16-byte units of a warp through shared memory (units rotated
+// by the row against bank conflicts), so that a store instruction covers whole segments
+// of 16 U bytes instead of 32 rows' 16 bytes.
+template <uint32_t U> __device__ __forceinline__ uint8_t *staged(uint8_t *buf, uint32_t row, uint32_t j)
 {
-    *reinterpret_cast<uint4 *>(buf + lane * 64 + ((j ^ (lane >> 1)) & 3u) * 16) = v;
+    return buf + (row * U + ((j ^ (U == 8 ? row : row >> 1)) & (U - 1))) * 16;
 }
 
-__device__ __forceinline__ uint4 stage_get(const uint8_t *buf, uint32_t row, uint32_t j)
+template <uint32_t U> __device__ __forceinline__ void stage_put(uint8_t *buf, uint32_t lane, uint32_t j, uint4 v)
 {
-    return *reinterpret_cast<const uint4 *>(buf + row * 64 + ((j ^ (row >> 1)) & 3u) * 16);
+    *reinterpret_cast<uint4 *>(staged<U>(buf, lane, j)) = v;
 }
 
-// The staged 64 bytes of rows [m, m + 32) below m_end, at byte `off` of rows of `pitch` bytes.
-__device__ __forceinline__ void stage_out(const uint8_t *buf, uint32_t lane, uint8_t *out, size_t pitch, size_t off, uint32_t m, uint32_t m_end)
+// The staged bytes of rows [m, m + 32) below m_end, at byte `off` of rows of `pitch` bytes.
+template <uint32_t U>
+__device__ __forceinline__ void stage_out(uint8_t *buf, uint32_t lane, uint8_t *out, size_t pitch, size_t off, uint32_t m, uint32_t m_end)
 {
     __syncwarp();
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t r = i * 8 + (lane >> 2), j = lane & 3;
-        const uint4 v = stage_get(buf, r, j);
+#pragma unroll (U == 8 ? 2 : 4)
+    for (uint32_t i = 0; i < U; ++i) {
+        const uint32_t r = i * (32 / U) + lane / U, j = lane & (U - 1);
+        const uint4 v = *reinterpret_cast<const uint4 *>(staged<U>(buf, r, j));
         if (m + r < m_end) *reinterpret_cast<uint4 *>(out + (size_t)(m + r) * pitch + off + j * 16) = v;
     }
     __syncwarp();
 }
 
 // A warp's 32 rows x 64 columns of C from column c: lane = row.
+template <uint32_t U>
 __device__ __forceinline__ void store_run(const Side &p, int out_f16, const float *acc, uint8_t *buf, uint32_t lane, uint32_t m, uint32_t m_end, uint32_t c)
 {
     const uint32_t size = out_f16 ? 2u : 4u;
@@ -347,23 +398,23 @@ __device__ __forceinline__ void store_run(const Side &p, int out_f16, const floa
         const size_t pitch = (size_t)p.N * size;
         if (out_f16) {
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
+            for (uint32_t h = 0; h < 8 / U; ++h) {
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const float *v = acc + 32 * h + 8 * j;
-                    stage_put(buf, lane, j, make_uint4(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]), half2_bits(v[4], v[5]), half2_bits(v[6], v[7])));
+                for (uint32_t j = 0; j < U; ++j) {
+                    const float *v = acc + 8 * (U * h + j);
+                    stage_put<U>(buf, lane, j, make_uint4(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]), half2_bits(v[4], v[5]), half2_bits(v[6], v[7])));
                 }
-                stage_out(buf, lane, out, pitch, (size_t)(c + 32 * h) * 2, m, m_end);
+                stage_out<U>(buf, lane, out, pitch, (size_t)(c + 8 * U * h) * 2, m, m_end);
             }
         } else {
 #pragma unroll
-            for (uint32_t h = 0; h < 4; ++h) {
+            for (uint32_t h = 0; h < 16 / U; ++h) {
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const float *v = acc + 16 * h + 4 * j;
-                    stage_put(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+                for (uint32_t j = 0; j < U; ++j) {
+                    const float *v = acc + 4 * (U * h + j);
+                    stage_put<U>(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
                 }
-                stage_out(buf, lane, out, pitch, (size_t)(c + 16 * h) * 4, m, m_end);
+                stage_out<U>(buf, lane, out, pitch, (size_t)(c + 4 * U * h) * 4, m, m_end);
             }
         }
         return;
@@ -374,14 +425,14 @@ __device__ __forceinline__ void store_run(const Side &p, int out_f16, const floa
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             const float *v = acc + 16 * h + 4 * j;
-            stage_put(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+            stage_put<4>(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
         }
         __syncwarp();
         const uint32_t cc = lane & 15, col = c + 16 * h + cc;
 #pragma unroll 4
         for (uint32_t i = 0; i < 16; ++i) {
             const uint32_t r = 2 * i + (lane >> 4);
-            const float v = *reinterpret_cast<const float *>(buf + r * 64 + (((cc >> 2) ^ (r >> 1)) & 3u) * 16 + (cc & 3) * 4);
+            const float v = *reinterpret_cast<const float *>(staged<4>(buf, r, cc >> 2) + (cc & 3) * 4);
             if (m + r < m_end && col < p.N) {
                 const size_t at = (size_t)(m + r) * p.N + col;
                 if (out_f16) static_cast<__half *>(p.out)[at] = __float2half_rn(v);
@@ -575,24 +626,45 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         // ------------------------------------------------ promotion and epilogue
         const uint32_t quarter = warp & 3, half = (uint32_t)(warp - 4) >> 2;
         const uint32_t lane_base = (quarter * 32u) << 16;
-        uint8_t *buf = smem + C::kOffOut + (warp - 4) * 2048;
+        uint8_t *buf = smem + C::kOffOut + (warp - 4) * C::kUnits * 512;
         uint32_t g = 0;
         bool alive = true;
+        // Scales a block ahead, and a tile's first before the epilogue of the tile before:
+        // taken over at the top of the next block, when their loads have had that time
+        // (the latter: 32 groups of 512 rows 259 against 268 us, 8192^3 515 against 521).
+        // run r: accumulator columns [64 half, + 64) of run r's 128
+        const float *sa = nullptr, *sb0 = nullptr, *sb1 = nullptr;
+        float an = 0.0f, u0n = 0.0f, u1n = 0.0f;
+        auto fetch = [&](uint32_t kk) {
+            an = __ldg(sa + kk);
+            u0n = __ldg(sb0 + kk);
+            if constexpr (kRuns == 2) u1n = __ldg(sb1 + kk);
+        };
+        const uint32_t warp_row = (MODE == PAIR ? rank * kBM : 0u) + quarter * 32;
+        auto begin = [&](uint32_t t) {
+            const Tile n = tile_at<C::kTileRows>(p, gr, t, kCols);
+            const Side &sd = p.side[n.side];
+            const uint32_t m = n.m0 + warp_row + lane, nblk = n.n0 / 128;
+            sa = sd.sa + (size_t)(m < n.m_end ? m : n.m0) * sd.kb;
+            sb0 = sd.sb0 + ((size_t)n.g * sd.nb + nblk) * sd.kb;
+            if (E == EPI_SWIGLU) sb1 = sd.sb1 + ((size_t)n.g * sd.nb + nblk) * sd.kb;
+            else sb1 = sb0 + (kRuns == 2 && nblk + 1 < sd.nb ? sd.kb : 0u);
+            fetch(k0);
+            return n;
+        };
+        Tile next{};
+        if (MODE != SPLIT && t0 < total) next = begin(t0);
         for (uint32_t t = t0; t < total && alive; t += step) {
-            const Tile tl = tile_at<C::kTileRows>(p, gr, t, kCols);
+            if (MODE == SPLIT) next = begin(t);
+            const Tile tl = next;
             const Side &sd = p.side[tl.side];
             const uint32_t k1 = k_end(sd);
-            const uint32_t m_warp = tl.m0 + (MODE == PAIR ? rank * kBM : 0u) + quarter * 32, m = m_warp + lane;
+            const uint32_t m_warp = tl.m0 + warp_row, m = m_warp + lane;
             const bool live = m_warp < tl.m_end;   // this warp has rows
             const bool row_ok = m < tl.m_end;
-            // run r: accumulator columns [64 half, + 64) of run r's 128
-            const uint32_t nblk = tl.n0 / 128, two = kRuns == 2 && (E == EPI_SWIGLU || nblk + 1 < sd.nb) ? 1u : 0u;
-            const float *sa = sd.sa + (size_t)(row_ok ? m : tl.m0) * sd.kb;
-            const float *sb0 = sd.sb0 + ((size_t)tl.g * sd.nb + nblk) * sd.kb;
-            const float *sb1 = E == EPI_SWIGLU ? sd.sb1 + ((size_t)tl.g * sd.nb + nblk) * sd.kb : sb0 + (size_t)two * sd.kb;
-            float acc[kRuns * 64];
+            uint64_t acc2[kRuns * 32];
 #pragma unroll
-            for (uint32_t i = 0; i < kRuns * 64; ++i) acc[i] = 0.0f;
+            for (uint32_t i = 0; i < kRuns * 32; ++i) acc2[i] = 0;
             // read out: the accumulator may be filled again
             auto release = [&](uint32_t b) {
                 tc_fence_before();
@@ -603,42 +675,24 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 }
             };
             if (live) {
-                // Scales a block ahead: taken over at the top of the next block, when their loads
-                // have had a whole block's time. One body, not unrolled: its code, the MMA
-                // issuer's and the producers' share the instruction cache.
-                float an = 0.0f, u0n = 0.0f, u1n = 0.0f;
-                auto fetch = [&](uint32_t kk) {
-                    if (kk < k1) {
-                        an = __ldg(sa + kk);
-                        u0n = __ldg(sb0 + kk);
-                        if constexpr (kRuns == 2) u1n = __ldg(sb1 + kk);
-                    }
-                };
-                fetch(k0);
+                // One body, not unrolled: its code, the MMA issuer's and the producers' share
+                // the instruction cache.
 #pragma unroll 1
                 for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
                     const float s0 = an * u0n, s1 = kRuns == 2 ? an * u1n : s0;
-                    fetch(kk + 1);
+                    if (kk + 1 < k1) fetch(kk + 1);
                     const uint32_t b = g % NA;
                     if (!wait_all(&acc_full[b], (g / NA) & 1u, abort, p.err, 0xF05)) { alive = false; break; }
                     tc_fence_after();
                     const uint32_t base = tmem + lane_base + b * BN + half * 64;
-                    uint32_t d[32], e[32];
-                    tmem_ld_32x32b_x32(base, d);
-                    tmem_ld_32x32b_x32(base + 32, e);
-                    tmem_ld_wait32(d);
-                    tmem_ld_wait32(e);
+                    uint64_t d[32];
+                    tmem_ld_pairs(base, d);
                     if constexpr (kRuns == 2) {
-                        promote32(acc, d, s0);
-                        promote32(acc + 32, e, s0);
-                        tmem_ld_32x32b_x32(base + 128, d);
-                        tmem_ld_32x32b_x32(base + 160, e);
-                        tmem_ld_wait32(d);
-                        tmem_ld_wait32(e);
+                        promote_pairs(acc2, d, dup2(s0));
+                        tmem_ld_pairs(base + 128, d);
                     }
                     release(b);
-                    promote32(acc + kRuns * 64 - 64, d, s1);
-                    promote32(acc + kRuns * 64 - 32, e, s1);
+                    promote_pairs(acc2 + kRuns * 32 - 32, d, dup2(s1));
                 }
             } else {
                 for (uint32_t kk = k0; kk < k1; ++kk, ++g) {
@@ -646,6 +700,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     release(g % NA);
                 }
             }
+            if (MODE != SPLIT && t + step < total) next = begin(t + step);
+            float acc[kRuns * 64];
+#pragma unroll
+            for (uint32_t i = 0; i < kRuns * 32; ++i) asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[2 * i]), "=f"(acc[2 * i + 1]) : "l"(acc2[i]));
             if (E != EPI_SWIGLU && !alive) break;
             if (MODE == SPLIT && parts > 1) {
                 // every copy has landed and every MMA has completed: the ring is free.
@@ -690,9 +748,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                             const float *v = acc + 16 * i + 4 * q;
                             w[q] = enc_f8x2(p.out_fmt, v[0] * inv, v[1] * inv) | enc_f8x2(p.out_fmt, v[2] * inv, v[3] * inv) << 16;
                         }
-                        stage_put(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
+                        stage_put<4>(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
                     }
-                    stage_out(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
+                    stage_out<4>(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
                     if (row_ok && half == 0) sd.out_scales[(size_t)m * sd.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
                 }
             } else if (live) {
@@ -704,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 #pragma unroll
                 for (uint32_t r = 0; r < kRuns; ++r) {
                     const uint32_t c = tl.n0 + r * 128 + half * 64;
-                    if (c < sd.N) store_run(sd, p.out_f16, acc + r * 64, buf, lane, m_warp, tl.m_end, c);
+                    if (c < sd.N) store_run<C::kUnits>(sd, p.out_f16, acc + r * 64, buf, lane, m_warp, tl.m_end, c);
                 }
             }
         }

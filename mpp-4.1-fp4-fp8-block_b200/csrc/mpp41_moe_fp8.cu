@@ -27,44 +27,57 @@ namespace fp8 {
 constexpr int kPlanThreads = 512;
 
 // Rows of expert e: one CTA reading all ids twice (they sit in L2): rows before e's = ids
-// below it, then a stable compaction. Threads own contiguous runs of assignments, so one
-// block scan orders them. No launch or wait joins the experts' CTAs.
+// below it, then a stable compaction. A warp owns a contiguous run of assignments, read in
+// chunks of 32 x 4, so one sum over the warps orders them; inside a chunk, which seldom
+// holds one of e's, lanes are ordered by a scan. No launch or wait joins the experts' CTAs.
 template <int THREADS>
 __device__ __forceinline__ void plan_expert(const int32_t *__restrict__ ids, const float *__restrict__ weights, uint32_t n, uint32_t E,
                                             int32_t e, int32_t *__restrict__ offsets, int32_t *__restrict__ inv,
                                             float *__restrict__ row_weight, uint32_t *err)
 {
-    __shared__ uint32_t sh_lt[THREADS / 32], sh_eq[THREADS / 32];
+    constexpr uint32_t kWarps = THREADS / 32;
+    __shared__ uint32_t sh_lt[kWarps], sh_eq[kWarps];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t per = (n + THREADS - 1) / THREADS;
-    const uint32_t a0 = min(threadIdx.x * per, n), a1 = min(a0 + per, n);
+    const uint32_t chunks = (n + 127) / 128, per = (chunks + kWarps - 1) / kWarps;
+    const uint32_t c0 = min(warp * per, chunks), c1 = min(c0 + per, chunks);
+    const bool vec = (reinterpret_cast<uintptr_t>(ids) & 15u) == 0;
+    auto load = [&](uint32_t c) {                       // this lane's four ids of a chunk, -1 behind the last
+        const uint32_t a = c * 128 + lane * 4;
+        if (vec && a + 4 <= n) return *reinterpret_cast<const int4 *>(ids + a);
+        return make_int4(a < n ? ids[a] : -1, a + 1 < n ? ids[a + 1] : -1, a + 2 < n ? ids[a + 2] : -1, a + 3 < n ? ids[a + 3] : -1);
+    };
+    auto equal = [&](const int4 &v) { return (v.x == e ? 1u : 0u) | (v.y == e ? 2u : 0u) | (v.z == e ? 4u : 0u) | (v.w == e ? 8u : 0u); };
     uint32_t lt = 0, eq = 0;
     bool bad = false;
-    for (uint32_t a = a0; a < a1; ++a) {
-        const int32_t id = ids[a];
-        lt += id >= 0 && id < e;
-        eq += id == e;
-        if (e == 0 && (id < 0 || id >= (int32_t)E)) {
-            inv[a] = -1;
-            bad |= id >= (int32_t)E;
+#pragma unroll 4
+    for (uint32_t c = c0; c < c1; ++c) {
+        const int4 v = load(c);
+        // unsigned: an id below 0 is above every expert
+        lt += ((uint32_t)v.x < (uint32_t)e) + ((uint32_t)v.y < (uint32_t)e) + ((uint32_t)v.z < (uint32_t)e) + ((uint32_t)v.w < (uint32_t)e);
+        eq += __popc(equal(v));
+        if (e == 0) {
+            const int32_t id[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t a = c * 128 + lane * 4 + j;
+                if (a < n && (uint32_t)id[j] >= E) {
+                    inv[a] = -1;
+                    bad |= id[j] >= 0;
+                }
+            }
         }
     }
     if (bad) report_error(err, kErrBounds, 0xF91);
-    uint32_t inc = eq;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= (uint32_t)o) inc += v;
-    }
     lt = __reduce_add_sync(0xffffffffu, lt);
-    if (lane == 31) {
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    if (lane == 0) {
         sh_lt[warp] = lt;
-        sh_eq[warp] = inc;
+        sh_eq[warp] = eq;
     }
     __syncthreads();
     uint32_t base = 0, all = 0, before = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < THREADS / 32; ++w) {
+    for (uint32_t w = 0; w < kWarps; ++w) {
         base += sh_lt[w];
         all += sh_eq[w];
         before += w < warp ? sh_eq[w] : 0u;
@@ -73,13 +86,27 @@ __device__ __forceinline__ void plan_expert(const int32_t *__restrict__ ids, con
         offsets[e] = (int32_t)base;
         if (e == (int32_t)E - 1) offsets[E] = (int32_t)(base + all);
     }
-    uint32_t row = base + before + inc - eq;
-    if (eq)
-        for (uint32_t a = a0; a < a1; ++a)
-            if (ids[a] == e) {
-                row_weight[row] = weights[a];
-                inv[a] = (int32_t)row++;
+    uint32_t row = base + before;
+    const uint32_t last = row + eq;
+    for (uint32_t c = c0; c < c1 && row < last; ++c) {
+        const uint32_t m = equal(load(c)), mine = __popc(m);
+        if (!__any_sync(0xffffffffu, m != 0)) continue;
+        uint32_t inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += v;
+        }
+        uint32_t r = row + inc - mine;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j)
+            if (m >> j & 1u) {
+                const uint32_t a = c * 128 + lane * 4 + j;
+                row_weight[r] = weights[a];
+                inv[a] = (int32_t)r++;
             }
+        row += __shfl_sync(0xffffffffu, inc, 31);
+    }
 }
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t *__restrict__ ids, const float *__restrict__ weights,
