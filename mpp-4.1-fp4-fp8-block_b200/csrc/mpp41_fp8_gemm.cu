@@ -91,7 +91,7 @@ cudaError_t launch(const Params &p, int dev, uint32_t grid, uint32_t parts, cuda
 namespace {
 
 // One side's fields; false when a tensor map cannot be made.
-bool fill(fp8::Side &d, const Fp8Launch &L, uint32_t cols, uint32_t box_rows)
+bool fill(fp8::Side &d, const Fp8Launch &L, uint32_t cols, uint32_t box_rows, bool boxes)
 {
     using namespace fp8;
     const bool swiglu = L.b1 != nullptr;
@@ -104,6 +104,8 @@ bool fill(fp8::Side &d, const Fp8Launch &L, uint32_t cols, uint32_t box_rows)
     const size_t row = (size_t)L.N * (swiglu ? 1 : L.out_f16 ? 2 : 4);
     d.vec = row % 16 == 0 && (reinterpret_cast<uintptr_t>(L.out) & 15u) == 0;
     const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    // where no tensor map can be made of C, it is stored without
+    d.boxes = boxes && !swiglu && d.vec && make_map(&d.tm_c, L.out, u8, 1, row, L.M, 128, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     const uint64_t b_rows = (uint64_t)L.groups * L.N;
     return make_map(&d.tm_a, L.a, u8, 1, L.K, L.M, kBK, box_rows, CU_TENSOR_MAP_SWIZZLE_128B) &&
            make_map(&d.tm_b0, L.b0, u8, 1, L.K, b_rows, kBK, 128, CU_TENSOR_MAP_SWIZZLE_128B) &&
@@ -135,7 +137,7 @@ int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
     memset(&p, 0, sizeof(p));
     // Copies of 32 rows where a group has few: 128 would bring its neighbours' rows too.
     p.box_rows = L.M / L.groups < 64 ? 32 : 128;
-    if (!fill(p.side[0], L, cols, p.box_rows) || (more && !fill(p.side[1], *more, cols, p.box_rows))) { *why = "tensor maps"; return 2; }
+    if (!fill(p.side[0], L, cols, p.box_rows, pair) || (more && !fill(p.side[1], *more, cols, p.box_rows, pair))) { *why = "tensor maps"; return 2; }
     p.offsets = L.offsets;
     p.groups = L.groups;
     p.all_groups = L.groups + (more ? 1 : 0);

@@ -65,13 +65,15 @@ template <int BN, int AR, int MODE> struct Cfg {
     static constexpr uint32_t kTileRows = MODE == PAIR ? 256 : 128;
     static constexpr uint32_t kAStage = AR * kBK;
     static constexpr uint32_t kBStage = (MODE == PAIR ? 1 : kRuns) * kBTile;   // PAIR: run `rank` only
-    static constexpr int kStages = MODE == PAIR ? 5 : BN == 256 ? 4 : (AR == 32 ? 9 : 6);
-    // 16-byte units of a staged output row. PAIR takes the sixth stage's room for 128-byte
-    // rows (4096 x 7168 x 2048, fp32 C: 77.7 against 81.3 us; one stage less costs nothing).
-    static constexpr uint32_t kUnits = MODE == PAIR ? 8 : 4;
+    static constexpr int kStages = BN == 256 ? 4 : (AR == 32 ? 9 : 6);
+    // PAIR: C leaves by bulk copies (store_boxes) from room that two more stages would take
+    // (6, 5 and 4 stages run alike). SINGLE's stages are larger, and with three of them 32
+    // groups of 512 rows took 258 us against 255, of 16 rows 77 against 75.
+    static constexpr bool kBoxes = MODE == PAIR;
+    static constexpr uint32_t kOutWarp = kBoxes ? 8192 : 2048;
     static constexpr uint32_t kOffB = ((kStages * kAStage + 1023) / 1024) * 1024;
-    static constexpr uint32_t kOffOut = kOffB + kStages * kBStage;  // 32 rows a promotion warp, epilogue transposition
-    static constexpr uint32_t kOffAmax = kOffOut + 8 * 512 * kUnits;        // SwiGLU: [2 halves][128] floats
+    static constexpr uint32_t kOffOut = kOffB + kStages * kBStage;  // kOutWarp a promotion warp: epilogue transposition
+    static constexpr uint32_t kOffAmax = kOffOut + 8 * kOutWarp;        // SwiGLU: [2 halves][128] floats
     static constexpr uint32_t kOffBar = kOffAmax + 1024;
     static constexpr uint32_t kOffGroups = kOffBar + 256;           // 3 words per group + 1
     static constexpr uint32_t kSmem = kOffGroups;                   // + group_bytes(all_groups)
@@ -93,7 +95,9 @@ struct Side {
     float *out_scales;          // SwiGLU: [M][nb]
     const float *row_scale;     // factor of each row of C, or null
     uint32_t M, N, kb, nb, n_tiles;
+    CUtensorMap tm_c;           // C [M][N] as bytes, box {128, 32}, SW128 (boxes)
     int vec;                    // rows of C start on 16-byte boundaries
+    int boxes;                  // tm_c is made
 };
 
 struct Params {
@@ -361,35 +365,44 @@ __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uin
     if (lane == 31) cum[p.all_groups] = inc;
 }
 
-// ---- epilogue: 32 rows of U 16-byte units of a warp through shared memory (units rotated
-// by the row against bank conflicts), so that a store instruction covers whole segments
-// of 16 U bytes instead of 32 rows' 16 bytes.
-template <uint32_t U> __device__ __forceinline__ uint8_t *staged(uint8_t *buf, uint32_t row, uint32_t j)
+// ---- epilogue: 32 rows x 64 bytes of a warp through shared memory (2 KB, 16-byte units
+// rotated by the row against bank conflicts), so that a store instruction covers eight
+// whole 64-byte row segments instead of 32 rows' 16 bytes.
+__device__ __forceinline__ uint8_t *staged(uint8_t *buf, uint32_t row, uint32_t j)
 {
-    return buf + (row * U + ((j ^ (U == 8 ? row : row >> 1)) & (U - 1))) * 16;
+    return buf + row * 64 + ((j ^ (row >> 1)) & 3u) * 16;
 }
 
-template <uint32_t U> __device__ __forceinline__ void stage_put(uint8_t *buf, uint32_t lane, uint32_t j, uint4 v)
+__device__ __forceinline__ void stage_put(uint8_t *buf, uint32_t lane, uint32_t j, uint4 v)
 {
-    *reinterpret_cast<uint4 *>(staged<U>(buf, lane, j)) = v;
+    *reinterpret_cast<uint4 *>(staged(buf, lane, j)) = v;
 }
 
-// The staged bytes of rows [m, m + 32) below m_end, at byte `off` of rows of `pitch` bytes.
-template <uint32_t U>
+// The staged 64 bytes of rows [m, m + 32) below m_end, at byte `off` of rows of `pitch` bytes.
 __device__ __forceinline__ void stage_out(uint8_t *buf, uint32_t lane, uint8_t *out, size_t pitch, size_t off, uint32_t m, uint32_t m_end)
 {
     __syncwarp();
-#pragma unroll (U == 8 ? 2 : 4)
-    for (uint32_t i = 0; i < U; ++i) {
-        const uint32_t r = i * (32 / U) + lane / U, j = lane & (U - 1);
-        const uint4 v = *reinterpret_cast<const uint4 *>(staged<U>(buf, r, j));
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t r = i * 8 + (lane >> 2), j = lane & 3;
+        const uint4 v = *reinterpret_cast<const uint4 *>(staged(buf, r, j));
         if (m + r < m_end) *reinterpret_cast<uint4 *>(out + (size_t)(m + r) * pitch + off + j * 16) = v;
     }
     __syncwarp();
 }
 
+// 16 bytes of a row of C from column v of its 64: 8 fp16 or 4 fp32 values.
+__device__ __forceinline__ uint4 unit_f16(const float *v)
+{
+    return make_uint4(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]), half2_bits(v[4], v[5]), half2_bits(v[6], v[7]));
+}
+
+__device__ __forceinline__ uint4 unit_f32(const float *v)
+{
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+
 // A warp's 32 rows x 64 columns of C from column c: lane = row.
-template <uint32_t U>
 __device__ __forceinline__ void store_run(const Side &p, int out_f16, const float *acc, uint8_t *buf, uint32_t lane, uint32_t m, uint32_t m_end, uint32_t c)
 {
     const uint32_t size = out_f16 ? 2u : 4u;
@@ -398,23 +411,17 @@ __device__ __forceinline__ void store_run(const Side &p, int out_f16, const floa
         const size_t pitch = (size_t)p.N * size;
         if (out_f16) {
 #pragma unroll
-            for (uint32_t h = 0; h < 8 / U; ++h) {
+            for (uint32_t h = 0; h < 2; ++h) {
 #pragma unroll
-                for (uint32_t j = 0; j < U; ++j) {
-                    const float *v = acc + 8 * (U * h + j);
-                    stage_put<U>(buf, lane, j, make_uint4(half2_bits(v[0], v[1]), half2_bits(v[2], v[3]), half2_bits(v[4], v[5]), half2_bits(v[6], v[7])));
-                }
-                stage_out<U>(buf, lane, out, pitch, (size_t)(c + 8 * U * h) * 2, m, m_end);
+                for (uint32_t j = 0; j < 4; ++j) stage_put(buf, lane, j, unit_f16(acc + 32 * h + 8 * j));
+                stage_out(buf, lane, out, pitch, (size_t)(c + 32 * h) * 2, m, m_end);
             }
         } else {
 #pragma unroll
-            for (uint32_t h = 0; h < 16 / U; ++h) {
+            for (uint32_t h = 0; h < 4; ++h) {
 #pragma unroll
-                for (uint32_t j = 0; j < U; ++j) {
-                    const float *v = acc + 4 * (U * h + j);
-                    stage_put<U>(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
-                }
-                stage_out<U>(buf, lane, out, pitch, (size_t)(c + 4 * U * h) * 4, m, m_end);
+                for (uint32_t j = 0; j < 4; ++j) stage_put(buf, lane, j, unit_f32(acc + 16 * h + 4 * j));
+                stage_out(buf, lane, out, pitch, (size_t)(c + 16 * h) * 4, m, m_end);
             }
         }
         return;
@@ -424,15 +431,14 @@ __device__ __forceinline__ void store_run(const Side &p, int out_f16, const floa
     for (uint32_t h = 0; h < 4; ++h) {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            const float *v = acc + 16 * h + 4 * j;
-            stage_put<4>(buf, lane, j, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+            stage_put(buf, lane, j, unit_f32(acc + 16 * h + 4 * j));
         }
         __syncwarp();
         const uint32_t cc = lane & 15, col = c + 16 * h + cc;
 #pragma unroll 4
         for (uint32_t i = 0; i < 16; ++i) {
             const uint32_t r = 2 * i + (lane >> 4);
-            const float v = *reinterpret_cast<const float *>(staged<4>(buf, r, cc >> 2) + (cc & 3) * 4);
+            const float v = *reinterpret_cast<const float *>(staged(buf, r, cc >> 2) + (cc & 3) * 4);
             if (m + r < m_end && col < p.N) {
                 const size_t at = (size_t)(m + r) * p.N + col;
                 if (out_f16) static_cast<__half *>(p.out)[at] = __float2half_rn(v);
@@ -440,6 +446,45 @@ __device__ __forceinline__ void store_run(const Side &p, int out_f16, const floa
             }
         }
         __syncwarp();
+    }
+}
+
+// The same for 32 whole rows, by bulk tensor copies that run on while the warp goes on
+// (4096 x 14336 x 4096: 219.5 against 221.6 us, 4096 x 7168 x 2048 in fp32: 74.3 against
+// 76.6): 128 bytes of every row (64 columns in fp16, 32 in fp32) into one of two slots, whose last
+// copy has been read by then. Columns behind the last are cut off by the tensor map.
+__device__ __forceinline__ void store_boxes(const Side &p, int out_f16, const float *acc, uint8_t *buf, uint32_t &boxes, uint32_t lane, uint32_t m, uint32_t c)
+{
+    auto slot = [&] {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+        return buf + (boxes & 1u) * 4096;
+    };
+    auto out = [&](const uint8_t *from, uint32_t byte) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0)
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n\t"
+                         "cp.async.bulk.commit_group;"
+                         ::"l"(&p.tm_c), "r"((int32_t)byte), "r"((int32_t)m), "r"(smem_u32(from))
+                         : "memory");
+        ++boxes;
+    };
+    if (out_f16) {
+        uint8_t *s = slot();
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) *reinterpret_cast<uint4 *>(s + lane * 128 + ((j ^ lane) & 7u) * 16) = unit_f16(acc + 8 * j);
+        out(s, c * 2);
+    } else {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            if (c + 32 * h >= p.N) break;
+            uint8_t *s = slot();
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                *reinterpret_cast<uint4 *>(s + lane * 128 + ((j ^ lane) & 7u) * 16) = unit_f32(acc + 32 * h + 4 * j);
+            out(s, (c + 32 * h) * 4);
+        }
     }
 }
 
@@ -626,7 +671,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         // ------------------------------------------------ promotion and epilogue
         const uint32_t quarter = warp & 3, half = (uint32_t)(warp - 4) >> 2;
         const uint32_t lane_base = (quarter * 32u) << 16;
-        uint8_t *buf = smem + C::kOffOut + (warp - 4) * C::kUnits * 512;
+        uint8_t *buf = smem + C::kOffOut + (warp - 4) * C::kOutWarp;
+        uint32_t boxes = 0;
         uint32_t g = 0;
         bool alive = true;
         // Scales a block ahead, and a tile's first before the epilogue of the tile before:
@@ -748,9 +794,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                             const float *v = acc + 16 * i + 4 * q;
                             w[q] = enc_f8x2(p.out_fmt, v[0] * inv, v[1] * inv) | enc_f8x2(p.out_fmt, v[2] * inv, v[3] * inv) << 16;
                         }
-                        stage_put<4>(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
+                        stage_put(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
                     }
-                    stage_out<4>(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
+                    stage_out(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
                     if (row_ok && half == 0) sd.out_scales[(size_t)m * sd.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
                 }
             } else if (live) {
@@ -759,13 +805,22 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 #pragma unroll
                     for (uint32_t i = 0; i < kRuns * 64; ++i) acc[i] *= f;
                 }
+                // groups end anywhere: a box that crosses the end would write the next group's rows
+                const bool whole = sd.boxes && m_warp + 32 <= tl.m_end;
+                if (C::kBoxes && !whole && boxes) {
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+                }
 #pragma unroll
                 for (uint32_t r = 0; r < kRuns; ++r) {
                     const uint32_t c = tl.n0 + r * 128 + half * 64;
-                    if (c < sd.N) store_run<C::kUnits>(sd, p.out_f16, acc + r * 64, buf, lane, m_warp, tl.m_end, c);
+                    if (c >= sd.N) break;
+                    if (C::kBoxes && whole) store_boxes(sd, p.out_f16, acc + r * 64, buf, boxes, lane, m_warp, c);
+                    else store_run(sd, p.out_f16, acc + r * 64, buf, lane, m_warp, tl.m_end, c);
                 }
             }
         }
+        if (C::kBoxes && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     // ---------------------------------------------------- teardown
