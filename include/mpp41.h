@@ -472,8 +472,8 @@ mpp41_status mpp41_moe_ep(mpp41_ctx *ctx, const mpp41_moe_desc *desc, uint32_t c
  *        renormalize (0 where that sum is 0: every chosen expert masked), times scale.
  *      Ties go to the lower index, of experts and of groups. The choice does not
  *      suffer from fp32 scores: without a bias experts (and groups by one expert) are
- *      compared by their logits, otherwise near ties are decided in 64 bits. Masked experts are
- *      chosen only where too few others are left, with weight 0.
+ *      compared by their logits, otherwise near ties are decided in 64 bits. Masked
+ *      experts are chosen only where too few others are left, with weight 0.
  *      experts <= 512; groups <= 32 divides experts; top_k <= 32 and at most
  *      top_groups * experts / groups. ---- */
 enum { MPP41_GATE_SOFTMAX = 0, MPP41_GATE_SIGMOID = 1 };
@@ -537,8 +537,8 @@ mpp41_status mpp41_matmul_fp8_grouped(mpp41_ctx *ctx, int a_fmt, const void *a, 
  *      (shared_intermediate > 0) one MLP of the same layout, its pointers NULL
  *      otherwise. out [tokens][hidden] fp32 or fp16, 16-byte aligned; for fp16 each
  *      weighted expert row (and the shared expert's) is rounded to fp16 before the fp32
- *      sum, whose own rounding it adds to (a row beyond 65504 is infinite). Sizes multiples
- *      of 128, experts <= 1024, top_k <= 32. scratch: mpp41_moe_fp8_scratch_bytes
+ *      sum, whose own rounding it adds to (a row beyond 65504 is infinite). Sizes
+ *      multiples of 128, experts <= 1024, top_k <= 32. scratch: mpp41_moe_fp8_scratch_bytes
  *      (0 for a descriptor that is refused), 256-byte aligned, its own for each call
  *      in flight. ---- */
 typedef struct {
