@@ -842,8 +842,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             const Tile tl = tile_at<C::kTileRows>(p, gr, t0, kCols);
             const Side &sd = p.side[0];
             const uint32_t rows = min(tl.m_end - tl.m0, kBM), base = smem_u32(smem);
-            // the cluster's CTAs take every parts-th 16-byte column of the tile, summed in rank order
-            for (uint32_t i = threadIdx.x * parts + rank; i < rows * (BN / 4); i += kThreads * parts) {
+            // the cluster's CTAs take a run of rows each, summed in rank order (interleaved
+            // columns share 32-byte sectors: 100 x 4096 x 2048 10.4 against 8.4 us)
+            const uint32_t i1 = rows * (rank + 1) / parts * (BN / 4);
+            for (uint32_t i = rows * rank / parts * (BN / 4) + threadIdx.x; i < i1; i += kThreads) {
                 const uint32_t r = i / (BN / 4), c4 = i % (BN / 4);
                 const uint32_t c = tl.n0 + 4 * c4;
                 if (c >= sd.N) continue;
