@@ -117,6 +117,8 @@ def check_product(got, a, b, k, f16):
     (5, 20000, 96), (260, 19000, 160), (4, 300, 14336),
     # pairs of CTAs: the odd one without rows, without columns, with neither
     (1100, 5120, 272), (1280, 4964, 144), (1100, 4964, 528),
+    # their bulk stores cut off behind the last column, in both types
+    (1100, 4968, 272), (1057, 5144, 128),
 ])
 def test_matmul(ctx, m, n, k, f16):
     rng = np.random.default_rng(m + n + k)
@@ -138,7 +140,8 @@ def test_matmul(ctx, m, n, k, f16):
 @pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("counts,n,k,tail", [
     ([5], 256, 256, 0), ([0, 0, 3, 0], 128, 128, 2), ([128, 1, 0, 130], 200, 272, 9), ([0, 0], 64, 64, 5),
-    ([300, 40, 7, 513, 1], 640, 512, 0), ([2500, 0, 700], 516, 400, 5), ([0], 300, 128, 1100), ([5, 4000], 256, 1040, 0), ([1] * 40, 130, 144, 1), ([0] * 31 + [64] + [2] * 100, 256, 128, 3),
+    ([300, 40, 7, 513, 1], 640, 512, 0), ([2500, 0, 700], 516, 400, 5), ([2500, 0, 700], 520, 400, 5), ([1501, 1030], 2088, 144, 3),
+    ([0], 300, 128, 1100), ([5, 4000], 256, 1040, 0), ([1] * 40, 130, 144, 1), ([0] * 31 + [64] + [2] * 100, 256, 128, 3),
 ])
 def test_grouped(ctx, counts, n, k, tail, f16):
     rng = np.random.default_rng(sum(counts) + n)

@@ -55,6 +55,8 @@ def setup(rng, h, i, e, shared, fmt):
 @pytest.mark.parametrize("t,h,i,e,k,shared,fmt,f16", [
     (1, 256, 128, 4, 2, 0, "e4m3", True), (1, 1024, 256, 8, 8, 128, "e4m3", False), (37, 384, 256, 6, 3, 384, "e5m2", True),
     (200, 512, 128, 3, 2, 0, "e4m3", False), (300, 256, 256, 40, 4, 256, "e4m3", True), (64, 128, 128, 1, 1, 0, "e5m2", False),
+    # pairs of CTAs (1024 rows an expert and more), beside a shared expert; more ids than one planning launch takes
+    (1200, 256, 256, 1, 1, 128, "e4m3", True), (2100, 384, 128, 2, 2, 256, "e5m2", False), (1501, 256, 128, 5, 3, 0, "e4m3", True),
 ])
 def test_layer(ctx, t, h, i, e, k, shared, fmt, f16):
     import mpp41
@@ -102,6 +104,30 @@ def test_ids_beyond_the_experts_are_reported(ctx):
     assert err.value.status == mpp41.ERR_BOUNDS
     ref = layer64(x, ids, w.astype(np.float64), ex, None, "e4m3")
     assert np.linalg.norm(out.cpu().numpy() - ref) <= 2e-3 * np.linalg.norm(ref)
+
+
+@pytest.mark.parametrize("t", [77, 1001])
+def test_ids_and_weights_at_any_element(ctx, t):
+    """Routing arrays that start on 4 bytes, not 16, and whose length no vector divides: the same bits."""
+    import mpp41
+    rng = np.random.default_rng(t)
+    h, i, e, k = 256, 128, 5, 3
+    dev, _, _, _ = setup(rng, h, i, e, 0, "e4m3")
+    x = torch.from_numpy(rng.standard_normal((t, h)).astype(np.float16)).cuda()
+    ids = torch.from_numpy(rng.integers(-1, e, t * k).astype(np.int32)).cuda()
+    w = torch.from_numpy(rng.random(t * k).astype(np.float32)).cuda()
+    desc = mpp41.moe_fp8_desc(t, h, i, e, k)
+    scratch = torch.empty(mpp41.moe_fp8_scratch_bytes(desc), dtype=torch.uint8, device="cuda")
+    outs = []
+    for off in (0, 1, 2, 3):
+        ids_at = torch.full((t * k + 8,), e + 7, dtype=torch.int32, device="cuda")
+        w_at = torch.full((t * k + 8,), float("nan"), device="cuda")
+        ids_at[off:off + t * k], w_at[off:off + t * k] = ids, w
+        out = torch.empty(t, h, device="cuda")
+        ctx.moe_fp8(desc, x, ids_at[off:], w_at[off:], *dev, out, scratch)
+        ctx.synchronize()
+        outs.append(out)
+    assert all(torch.equal(outs[0], o) for o in outs[1:]) and torch.isfinite(outs[0]).all()
 
 
 def test_all_padded_gives_zeros(ctx):
