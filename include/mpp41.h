@@ -535,9 +535,8 @@ mpp41_status mpp41_matmul_fp8_grouped(mpp41_ctx *ctx, int a_fmt, const void *a, 
  *      [experts][intermediate][hidden] with scales [experts][intermediate/128]
  *      [hidden/128], wd [experts][hidden][intermediate]; the shared expert
  *      (shared_intermediate > 0) one MLP of the same layout, its pointers NULL
- *      otherwise. out [tokens][hidden] fp32 or fp16, 16-byte aligned; for fp16 each
- *      weighted expert row (and the shared expert's) is rounded to fp16 before the fp32
- *      sum, whose own rounding it adds to (a row beyond 65504 is infinite). Sizes
+ *      otherwise. out [tokens][hidden] fp32 or fp16, 16-byte aligned: the weighted
+ *      rows are kept and summed in fp32, an fp16 out is rounded from the sum. Sizes
  *      multiples of 128, experts <= 1024, top_k <= 32. scratch: mpp41_moe_fp8_scratch_bytes
  *      (0 for a descriptor that is refused), 256-byte aligned, its own for each call
  *      in flight. ---- */

@@ -168,7 +168,7 @@ struct MoeFp8Layout {
 MoeFp8Layout moe_fp8_layout(const mpp41_moe_fp8_desc *d)
 {
     const size_t T = d->tokens, H = d->hidden, I = d->intermediate, R = T * d->top_k, Is = d->shared_intermediate;
-    const size_t Ts = Is ? T : 0, out_size = d->out_f16 ? 2 : 4;
+    const size_t Ts = Is ? T : 0;
     MoeFp8Layout l;
     size_t o = 0;
     auto part = [&](size_t bytes) { const size_t at = o; o += up256(bytes); return at; };
@@ -179,12 +179,12 @@ MoeFp8Layout moe_fp8_layout(const mpp41_moe_fp8_desc *d)
     l.ps = part(R * (H / 128) * 4);
     l.mq = part(R * I);
     l.ms = part(R * (I / 128) * 4);
-    l.y = part(R * H * out_size);
+    l.y = part(R * H * 4);
     l.xq = part(Ts * H);
     l.xs = part(Ts * (H / 128) * 4);
     l.smq = part(Ts * Is);
     l.sms = part(Ts * (Is / 128) * 4);
-    l.sy = part(Ts * H * out_size);
+    l.sy = part(Ts * H * 4);
     l.total = o;
     return l;
 }
@@ -256,7 +256,6 @@ mpp41_status mpp41_moe_fp8(mpp41_ctx *ctx, const mpp41_moe_fp8_desc *d, const vo
     n.out = b + l.y; n.out_scales = nullptr;
     n.row_scale = f32(l.rw);
     n.N = H; n.K = I;
-    n.out_f16 = d->out_f16 != 0;
     if (Is) {
         gs = g;
         gs.a = b + l.xq; gs.sa = f32(l.xs);
@@ -277,7 +276,7 @@ mpp41_status mpp41_moe_fp8(mpp41_ctx *ctx, const mpp41_moe_fp8_desc *d, const vo
     if (s != MPP41_OK) return s;
     s = run_gemm(n, st, "expert down product");
     if (s != MPP41_OK) return s;
-    return cuda_status(launch_fp8_combine(b + l.y, inv, T, k, H, Is ? b + l.sy : nullptr, out, d->out_f16 != 0, st), "combine");
+    return cuda_status(launch_fp8_combine(f32(l.y), inv, T, k, H, Is ? f32(l.sy) : nullptr, out, d->out_f16 != 0, st), "combine");
 }
 
 }  // extern "C"

@@ -160,7 +160,7 @@ cudaError_t launch_quantize_weights_fp8(int fmt, const float *w, uint32_t N, uin
 cudaError_t launch_fp8_scatter(int fmt, const int32_t *ids, const float *weights, uint32_t E, int32_t *offsets, int32_t *inv,
                                float *row_weight, uint32_t *err, const void *x, uint32_t T, uint32_t H, uint32_t k, uint8_t *pq,
                                float *ps, uint8_t *xq, float *xs, cudaStream_t st);
-cudaError_t launch_fp8_combine(const void *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const void *shared_y,
+cudaError_t launch_fp8_combine(const float *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const float *shared_y,
                                void *out, int f16, cudaStream_t st);
 
 // Expert routing with scores, balance bias and groups (mpp41_moe_gate.cu): E <= 512,

@@ -9,9 +9,10 @@
 //             the grouped down product, each row times its routing weight
 //             -> y [rows][H]; the shared expert's tiles run in the same two launches.
 //   combine:  out[t] = shared(t) + sum_j y[inv[t*k+j]], in slot order, summed in fp32.
-// y has out's type. For fp16 out the weighted rows are rounded to fp16 (2^-11 of each
-// term, as the sum's own rounding; terms beyond 65504 need a sum that is too): half the
-// bytes between the products and the combine, which at 2000 tokens are 0.9 GB in fp32.
+// y and the shared expert's rows are fp32 whatever out's type: terms of opposite sign may
+// cancel, and two of more than 65504 leave a finite sum that fp16 rows would lose. An fp16
+// out is rounded once, from the sum. (fp16 rows: 1020 against 1093 us for 2048 tokens of
+// the 7168 / 2048 layer, 8 of 32 experts; no difference for one token.)
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -214,51 +215,35 @@ __global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t *__rest
 constexpr int kCombineThreads = 128;
 
 template <bool F16>
-__global__ void __launch_bounds__(kCombineThreads) combine_fp8_kernel(const uint4 *__restrict__ y, const int32_t *__restrict__ inv,
-                                                                      uint32_t k, uint32_t row16,
-                                                                      const uint4 *__restrict__ shared_y, uint4 *__restrict__ out)
+__global__ void __launch_bounds__(kCombineThreads) combine_fp8_kernel(const float4 *__restrict__ y, const int32_t *__restrict__ inv,
+                                                                      uint32_t k, uint32_t units,
+                                                                      const float4 *__restrict__ shared_y, void *__restrict__ out)
 {
-    constexpr int V = F16 ? 8 : 4;
     __shared__ int32_t rows[32];
     const uint32_t t = blockIdx.x, c = blockIdx.y * kCombineThreads + threadIdx.x;
     if (threadIdx.x < k) rows[threadIdx.x] = inv[(size_t)t * k + threadIdx.x];
-    uint4 sh = make_uint4(0, 0, 0, 0);
-    if (shared_y && c < row16) sh = __ldcs(shared_y + (size_t)t * row16 + c);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (shared_y && c < units) acc = __ldcs(shared_y + (size_t)t * units + c);
     __syncthreads();
-    if (c >= row16) return;
-    float acc[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    auto add = [&](const uint4 &v) {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (F16) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                acc[(2 * i) % V] += f.x;
-                acc[(2 * i + 1) % V] += f.y;
-            } else {
-                acc[i] += __uint_as_float(w[i]);
-            }
-        }
-    };
-    add(sh);
+    if (c >= units) return;
     for (uint32_t j0 = 0; j0 < k; j0 += 8) {
-        uint4 v[8];
+        float4 v[8];
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
             const int32_t r = j0 + j < k ? rows[j0 + j] : -1;
-            v[j] = r >= 0 ? __ldcs(y + (size_t)r * row16 + c) : make_uint4(0, 0, 0, 0);
+            v[j] = r >= 0 ? __ldcs(y + (size_t)r * units + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) add(v[j]);
+        for (uint32_t j = 0; j < 8; ++j) {
+            acc.x += v[j].x;
+            acc.y += v[j].y;
+            acc.z += v[j].z;
+            acc.w += v[j].w;
+        }
     }
-    uint4 o;
-    if (F16)
-        o = make_uint4(half2_bits(acc[0], acc[1]), half2_bits(acc[2], acc[3]), half2_bits(acc[4 % V], acc[5 % V]), half2_bits(acc[6 % V], acc[7 % V]));
-    else
-        o = make_uint4(__float_as_uint(acc[0]), __float_as_uint(acc[1]), __float_as_uint(acc[2]), __float_as_uint(acc[3]));
-    out[(size_t)t * row16 + c] = o;
+    const size_t at = (size_t)t * units + c;
+    if (F16) static_cast<uint2 *>(out)[at] = make_uint2(half2_bits(acc.x, acc.y), half2_bits(acc.z, acc.w));
+    else static_cast<float4 *>(out)[at] = acc;
 }
 
 }  // namespace fp8
@@ -290,14 +275,14 @@ cudaError_t launch_fp8_scatter(int fmt, const int32_t *ids, const float *weights
     return cudaGetLastError();
 }
 
-cudaError_t launch_fp8_combine(const void *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const void *shared_y,
+cudaError_t launch_fp8_combine(const float *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const float *shared_y,
                                void *out, int f16, cudaStream_t st)
 {
-    const uint32_t row16 = H / (f16 ? 8 : 4);
-    const dim3 grid(T, (row16 + fp8::kCombineThreads - 1) / fp8::kCombineThreads);
-    const uint4 *a = static_cast<const uint4 *>(y), *sy = static_cast<const uint4 *>(shared_y);
-    if (f16) fp8::combine_fp8_kernel<true><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
-    else fp8::combine_fp8_kernel<false><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, row16, sy, static_cast<uint4 *>(out));
+    const uint32_t units = H / 4;
+    const dim3 grid(T, (units + fp8::kCombineThreads - 1) / fp8::kCombineThreads);
+    const float4 *a = reinterpret_cast<const float4 *>(y), *sy = reinterpret_cast<const float4 *>(shared_y);
+    if (f16) fp8::combine_fp8_kernel<true><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, units, sy, out);
+    else fp8::combine_fp8_kernel<false><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, units, sy, out);
     return cudaGetLastError();
 }
 
