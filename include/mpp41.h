@@ -526,11 +526,11 @@ mpp41_status mpp41_matmul_fp8_grouped(mpp41_ctx *ctx, int a_fmt, const void *a, 
 /* ---- expert layer in FP8 (W8A8 with the scales above), the routing given:
  *        out[t] = shared_expert(x[t]) + sum_j weights[t][j] * expert_{ids[t][j]}(x[t])
  *      over j < top_k in order; expert(x) = down(q(silu(gate(q(x))) * up(q(x)))) with
- *      q the 1 x 128 activation quantizer (the mid in fp32 before it). A negative id
- *      is no expert and adds nothing (a padded token, an expert of another rank); an
- *      id of experts or more adds nothing either and is reported as
- *      MPP41_ERR_BOUNDS by mpp41_synchronize. The same id twice in a token counts
- *      twice. x fp16 [tokens][hidden], 32-byte aligned; ids and weights
+ *      q the 1 x 128 activation quantizer (the mid in fp32 before it, where infinities
+ *      count as the largest finite value). A negative id is no expert and adds nothing
+ *      (a padded token, an expert of another rank); an id of experts or more adds
+ *      nothing either and is reported as MPP41_ERR_BOUNDS by mpp41_synchronize. The
+ *      same id twice in a token counts twice. x fp16 [tokens][hidden], 32-byte aligned; ids and weights
  *      [tokens][top_k] as mpp41_moe_gate writes them; weights of `fmt`: wg, wu
  *      [experts][intermediate][hidden] with scales [experts][intermediate/128]
  *      [hidden/128], wd [experts][hidden][intermediate]; the shared expert

@@ -281,6 +281,17 @@ __device__ __forceinline__ uint64_t dup2(float s)
     return r;
 }
 
+// g / (1 + e^-g) within 10 * 2^-24 of its size: expf (1 ulp), the sum, the reciprocal (2^-23)
+// and a product; 0 below -88.7, where e^-g is infinite. Taken at a quarter of its size the
+// divisor has a normal reciprocal over the whole range. (__expf is off by |g| 2^-23 more;
+// a division instead of the reciprocal: 332 against 301 us for the layer of 128 tokens.)
+__device__ __forceinline__ float silu(float g)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(expf(-g), 0.25f, 0.25f)));
+    return 0.25f * g * r;
+}
+
 // Barrier of the promotion warps that also ORs a flag.
 __device__ __forceinline__ bool promo_any(bool v)
 {
@@ -771,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 if (live) {
 #pragma unroll
                     for (uint32_t i = 0; i < 64; ++i) {
-                        acc[i] = __fdividef(acc[i], 1.0f + __expf(-acc[i])) * acc[64 + i];
+                        acc[i] = silu(acc[i]) * acc[64 + i];
                         vmax = fmaxf(vmax, fabsf(acc[i]));
                     }
                 }
@@ -782,22 +793,23 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 vmax = fmaxf(amax_x[r], amax_x[128 + r]);
                 asm volatile("barrier.sync 1, %0;" ::"n"(kPromoThreads) : "memory");   // before the next tile's write
                 if (live) {
-                    // below 1e-30 the group is zero for every output type; the floor keeps qmax / vmax finite
-                    vmax = fminf(fmaxf(vmax, 1.0e-30f), 3.0e38f);
-                    const float qmax = f8_max(p.out_fmt);
-                    const float inv = __fdiv_rn(qmax, vmax);
+                    // as the activation quantizer: scale 1 where all is zero, infinities as the largest
+                    // finite value. Blocks so small that qmax / vmax would overflow are raised first.
+                    vmax = fminf(vmax, 3.402823466e38f);
+                    const float qmax = f8_max(p.out_fmt), raise = vmax < 0x1p-100f ? 0x1p100f : 1.0f;
+                    const float inv = vmax > 0.0f ? __fdiv_rn(qmax, vmax * raise) : 0.0f;
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i) {
                         uint32_t w[4];
 #pragma unroll
                         for (uint32_t q = 0; q < 4; ++q) {
                             const float *v = acc + 16 * i + 4 * q;
-                            w[q] = enc_f8x2(p.out_fmt, v[0] * inv, v[1] * inv) | enc_f8x2(p.out_fmt, v[2] * inv, v[3] * inv) << 16;
+                            w[q] = enc_f8x2(p.out_fmt, v[0] * raise * inv, v[1] * raise * inv) | enc_f8x2(p.out_fmt, v[2] * raise * inv, v[3] * raise * inv) << 16;
                         }
                         stage_put(buf, lane, i, make_uint4(w[0], w[1], w[2], w[3]));
                     }
                     stage_out(buf, lane, static_cast<uint8_t *>(sd.out), sd.N, tl.n0 + half * 64, m_warp, tl.m_end);
-                    if (row_ok && half == 0) sd.out_scales[(size_t)m * sd.nb + tl.n0 / 128] = __fdiv_rn(vmax, qmax);
+                    if (row_ok && half == 0) sd.out_scales[(size_t)m * sd.nb + tl.n0 / 128] = vmax > 0.0f ? __fdiv_rn(vmax, qmax) : 1.0f;
                 }
             } else if (live) {
                 if (sd.row_scale) {
