@@ -640,6 +640,11 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         if (MODE != PAIR || rank == 0)
             for (uint32_t q = (g > (uint32_t)S ? g - S : 0); q < g; ++q)
                 mbar_wait(&full[q % S], (q / S) & 1u, nullptr, p.err, 0xF02);
+        // PAIR: the even CTA's commits arrive here too, the last round of them unasked for; a CTA
+        // that left before they land would have them written into its successor's memory
+        if (MODE == PAIR && is_b && alive)
+            for (uint32_t q = (g > (uint32_t)S ? g - S : 0); q < g; ++q)
+                mbar_wait(&empty[q % S], (q / S) & 1u, nullptr, p.err, 0xF07);
       } else if (warp == 1 && (MODE != PAIR || rank == 0)) {
         // ------------------------------------------------ MMA issuer
         const uint64_t ad0 = smem_desc_sw128(sA), bd0 = smem_desc_sw128(sB);
@@ -838,7 +843,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     // ---------------------------------------------------- teardown
     tc_fence_before();
     __syncthreads();
-    if (warp == 1 && (MODE != PAIR || rank == 0)) mbar_wait(drain, 0, nullptr, p.err, 0xF06);   // every issued MMA has completed
+    // every issued MMA has completed (PAIR: the even CTA's last commit arrives in both)
+    if (warp == 1) mbar_wait(drain, 0, nullptr, p.err, 0xF06);
     __syncthreads();
     // PAIR: neither CTA leaves while the other arrives on its barriers or the MMAs
     // read its memory. SPLIT: the partials are complete.
