@@ -509,8 +509,9 @@ mpp41_status mpp41_moe_gate(mpp41_ctx *ctx, const mpp41_gate_desc *desc, const v
  *      - mpp41_matmul_fp8_grouped: rows [offsets[g], offsets[g+1]) of A and C with
  *        B[g], B [groups][N][K], its scales [groups][ceil(N/128)][ceil(K/128)];
  *        offsets [groups + 1] on the device, ascending within [0, M] (others are
- *        clamped and reported as MPP41_ERR_BOUNDS by mpp41_synchronize). Rows of C
- *        outside the groups are left as they are. groups <= 1024.
+ *        clamped to [0, M], raised to the largest before them and reported as
+ *        MPP41_ERR_BOUNDS by mpp41_synchronize). Rows of C outside the groups are
+ *        left as they are. groups <= 1024.
  *      K a positive multiple of 16; M, groups * N and K below 2^31; A and B 16-byte
  *      aligned. Results do not depend on the run: sums have a fixed order. ---- */
 mpp41_status mpp41_quantize_act_fp8(mpp41_ctx *ctx, int fmt, const void *x, uint32_t tokens, uint32_t hidden,

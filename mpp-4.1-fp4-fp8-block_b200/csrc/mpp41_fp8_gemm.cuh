@@ -336,25 +336,44 @@ __device__ __forceinline__ Tile tile_at(const Params &p, const Groups &gr, uint3
     return o;
 }
 
-// Prefix sums of the groups' tiles (one warp). Offsets are clamped to [0, M] and made
-// ascending, so wrong ones are reported but never lead out of A or C.
+// Prefix sums of the groups' tiles (one warp). Offsets are clamped to [0, M] and raised to
+// the largest before them: wrong ones are reported, lead nowhere out of A or C, and give
+// every row to one group at most.
 template <uint32_t ROWS>
 __device__ __forceinline__ void build_groups(const Params &p, uint32_t *cum, uint32_t *row0, uint32_t *row1, uint32_t lane)
 {
     const uint32_t per = (p.all_groups + 31) / 32;
     auto tiles = [&](uint32_t g) { return (row1[g] - row0[g] + ROWS - 1) / ROWS * p.side[g == p.groups].n_tiles; };
-    uint32_t sum = 0;
+    uint32_t sum = 0, least = 0;   // least: the largest start of the groups before
     bool bad = false;
+    if (p.offsets) {
+        uint32_t most = 0;
+        for (uint32_t i = 0; i < per; ++i) {
+            const uint32_t g = lane * per + i;
+            if (g >= p.groups) break;
+            const int32_t o0 = p.offsets[g], o1 = p.offsets[g + 1], m = (int32_t)p.side[0].M;
+            const int32_t a = min(max(o0, 0), m), b = min(max(o1, 0), m);
+            bad |= a != o0 || b != o1;
+            row0[g] = (uint32_t)a;
+            row1[g] = (uint32_t)b;
+            most = max(most, (uint32_t)a);
+        }
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, most, o);
+            if (lane >= (uint32_t)o) most = max(most, v);
+        }
+        least = __shfl_up_sync(0xffffffffu, most, 1);
+        if (lane == 0) least = 0;
+    }
     for (uint32_t i = 0; i < per; ++i) {
         const uint32_t g = lane * per + i;
         if (g >= p.all_groups) break;
         uint32_t a = 0, b = p.side[g == p.groups].M;
         if (p.offsets && g < p.groups) {
-            const int32_t o0 = p.offsets[g], o1 = p.offsets[g + 1];
-            const int64_t m = p.side[0].M;
-            a = (uint32_t)min(max((int64_t)o0, (int64_t)0), m);
-            b = (uint32_t)min(max((int64_t)o1, (int64_t)a), m);
-            bad |= (int64_t)a != o0 || (int64_t)b != o1;
+            a = max(row0[g], least);
+            b = max(row1[g], a);
+            bad |= a != row0[g] || b != row1[g];
+            least = a;
         }
         row0[g] = a;
         row1[g] = b;
