@@ -23,7 +23,6 @@ template <int FMT>
 __global__ void __launch_bounds__(256) quant_act_kernel(const uint8_t *__restrict__ x, uint32_t H, uint32_t kb,
                                                         uint64_t blocks, uint8_t *__restrict__ q, float *__restrict__ scales)
 {
-    pdl_launch_dependents();
     pdl_wait_prior();
     const uint32_t sub = threadIdx.x & 7;
     const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 8);
@@ -48,7 +47,6 @@ template <int FMT>
 __global__ void __launch_bounds__(256) quant_act_any_kernel(const __half *__restrict__ x, uint32_t H, uint32_t kb,
                                                             uint64_t blocks, uint8_t *__restrict__ q, float *__restrict__ scales)
 {
-    pdl_launch_dependents();
     pdl_wait_prior();
     const uint32_t lane = threadIdx.x & 31;
     const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 32);
@@ -84,7 +82,6 @@ __global__ void __launch_bounds__(512, 2) quant_weights_kernel(const float *__re
                                                             uint8_t *__restrict__ q, float *__restrict__ scales)
 {
     __shared__ float part[16];
-    pdl_launch_dependents();
     pdl_wait_prior();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t bn = blockIdx.x / kb, bk = blockIdx.x - bn * kb;

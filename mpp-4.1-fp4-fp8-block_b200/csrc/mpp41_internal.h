@@ -109,8 +109,10 @@ struct MxLaunch {
 };
 int launch_mxf4_gemm(const MxLaunch &L, cudaStream_t st, const char **why);
 
-// Launch whose start overlaps the end of the kernel before it on the stream; the kernel
-// calls pdl_wait_prior() before it touches global memory.
+// Launch whose start overlaps the end of the kernel before it on the stream, where that one
+// lets it; the kernel calls pdl_wait_prior() before it touches global memory. It does not
+// let the next one start early itself: the MLP kernels stream their weights before they
+// wait, and what such a kernel writes may be those weights.
 template <typename... K, typename... A>
 cudaError_t launch_overlapped(void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args)
 {

@@ -315,7 +315,6 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double *sv = smem + (size_t)warp * p.E;
     const uint32_t stride = gridDim.x * kWarps * batch;
-    pdl_launch_dependents();
     pdl_wait_prior();
     float bias[PER];
 #pragma unroll
