@@ -466,7 +466,7 @@ mpp41_status mpp41_moe_ep(mpp41_ctx *ctx, const mpp41_moe_desc *desc, uint32_t c
  *        s = softmax(z) or sigmoid(z);  v = s + bias (bias [experts] fp32, or NULL).
  *        A logit of -inf or NaN masks its expert: s = 0, v = -inf (a NaN sum too).
  *        The experts form `groups` equal runs; a group's worth is the sum of its
- *        group_top (1 or 2) largest v; the top_groups best groups stay.
+ *        group_top (1 or 2) largest v (inf - inf: -inf); the top_groups best groups stay.
  *        ids[t][0..top_k) = the experts of those groups by falling v;
  *        weights[t][j] = s of that expert, over the sum of the chosen with
  *        renormalize (0 where that sum is 0: every chosen expert masked), times scale.

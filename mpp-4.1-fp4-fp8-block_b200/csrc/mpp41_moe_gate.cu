@@ -148,7 +148,8 @@ __device__ __noinline__ uint32_t exact_token(const Params &p, size_t row, uint32
             b1 = fmax(fmin(b0, o0), fmax(b1, o1));
             b0 = fmax(b0, o0);
         }
-        const double worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
+        double worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
+        if (!(worth > -inf)) worth = -inf;   // inf - inf
         uint32_t rank = 0;
 #pragma unroll 4
         for (uint32_t i = 0; i < p.groups; ++i) {
@@ -400,7 +401,9 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
                     b1 = fmaxf(fminf(b0, o0), fmaxf(b1, o1));
                     b0 = fmaxf(b0, o0);
                 }
-                const float worth = p.group_top == 2 && p.group_size > 1 ? b0 + b1 : b0;
+                const bool two = p.group_top == 2 && p.group_size > 1;
+                float worth = two ? b0 + b1 : b0;
+                if (!(worth > -INFINITY)) worth = -INFINITY;   // inf - inf
                 uint32_t rank = 0;
                 if (!p.scores) {
                     for (uint32_t g = 0; g < p.groups; ++g) {
@@ -422,12 +425,15 @@ __global__ void __launch_bounds__(32 * kWarps, PER <= 8 ? 7 : 5) fast_kernel(con
                     for (uint32_t g = 0; g < p.groups; ++g) stay |= (in_lanes >> (g * lanes) & 1u) << g;
                 }
                 if (p.scores) {
-                    // the last group that stays and the first that goes have to be well apart
-                    const uint32_t k = order_bits(worth);
-                    const float in = order_value(__reduce_min_sync(kFull, keep ? k : 0xFFFFFFFFu));
-                    const float out = order_value(__reduce_max_sync(kFull, real && !keep ? k : 0u));
-                    sure = __popc(in_lanes) == p.top_groups * lanes &&
-                           in - out > 2.0f * err + fabsf(in) * (1.0f / 4194304.0f);   // sums of two
+                    // The last group that stays and the first that goes have to be well apart.
+                    // A worth is off by its scores' errors (err covers two) and by half an ulp of
+                    // each addend and of the sum, whose own size says nothing of theirs where
+                    // they have opposite signs: 2^-23 of both addends' sizes, here 2^-22.
+                    const float far = err + (fabsf(b0) + (two ? fabsf(b1) : 0.0f)) * (1.0f / 4194304.0f);
+                    const float off = fabsf(worth) < INFINITY ? far : 0.0f;   // infinite worths are exact
+                    const float in = order_value(__reduce_min_sync(kFull, keep ? order_bits(worth - off) : 0xFFFFFFFFu));
+                    const float out = order_value(__reduce_max_sync(kFull, real && !keep ? order_bits(worth + off) : 0u));
+                    sure = __popc(in_lanes) == p.top_groups * lanes && in > out;
                 }
             }
             uint32_t key[PER];
