@@ -497,9 +497,8 @@ mpp41_status mpp41_moe_gate(mpp41_ctx *ctx, const mpp41_gate_desc *desc, const v
  *        as +-65504; NaN stays NaN and does not enter amax.
  *      - mpp41_quantize_weights_fp8: fp32 w [rows][depth] -> q [rows][depth], scales
  *        [ceil(rows/128)][ceil(depth/128)]: per 128 x 128, scale = amax / qmax,
- *        q = w * (qmax / amax) in fp32 (blocks whose amax is below 1e-30:
- *        (w / amax) * qmax), rounded to nearest even. Infinities count as the largest
- *        finite value; NaN as above.
+ *        q = w * qmax / amax correctly rounded to nearest even. Infinities count as the
+ *        largest finite value; NaN as above.
  *      Any sizes; buffers aligned to their elements (x 32-byte and q 16-byte aligned
  *      with hidden % 16 == 0, or w 16-byte with depth % 4 == 0, runs wide accesses).
  *      - mpp41_matmul_fp8: C[M][N] = A[M][K] B[N][K]^T, A with scales [M][ceil(K/128)],

@@ -72,11 +72,27 @@ __global__ void __launch_bounds__(256) quant_act_any_kernel(const __half *__rest
     }
 }
 
+// round(w * qmax / amax), exactly: 7 w and m * amax, m a midpoint of the
+// 8-bit format (5 bits), are integers of 27 and 29 bits, so the quotient is a midpoint or at
+// least 2^-30 of its size away from one, which 64 bits tell apart. The quotient reaches the
+// encoder as fp32 cut to zero, its lowest bit set where anything was cut: a value next to a
+// midpoint stays on its side.
+template <int FMT> __device__ __forceinline__ uint8_t exact_f8(float w, float amax)
+{
+    const double d = (double)w * (double)f8_max(FMT) / (double)amax;
+    float f = __double2float_rz(d);
+    if ((double)f != d) f = __uint_as_float(__float_as_uint(f) | 1u);
+    return (uint8_t)enc_f8x2(FMT, f, 0.0f);
+}
+
 // One CTA a 128 x 128 block, 32 fp32 values a thread (two CTAs an SM, so that one's loads
 // cover another's stores): warp w has rows w, w + 16, ..., a lane four neighbouring columns
 // (VEC: K % 4 == 0 and aligned pointers).
-// q = round(w * (qmax / amax)), two fp32 roundings: 14336 x 4096 in 48 us, 93 % of the
-// copy rate; with a division a value 57 us.
+// q = round(w * qmax / amax), correctly rounded: fp32 products with a factor 2^-21 below and
+// one as far above the quotient, which their three roundings (2^-24 each) do not bridge. Where
+// both give the same code it is the exact quotient's, elsewhere (one value in 10^5) 64 bits
+// decide: 14336 x 4096 in 48.3 us, 93 % of the copy rate (48.0 with one rounded factor and
+// wrong codes at some midpoints, 57 with a division a value).
 template <int FMT, bool VEC>
 __global__ void __launch_bounds__(512, 2) quant_weights_kernel(const float *__restrict__ w, uint32_t N, uint32_t K, uint32_t kb,
                                                             uint8_t *__restrict__ q, float *__restrict__ scales)
@@ -115,20 +131,19 @@ __global__ void __launch_bounds__(512, 2) quant_weights_kernel(const float *__re
     for (int j = 0; j < 16; ++j) amax = fmaxf(amax, part[j]);
     amax = fminf(amax, 3.402823466e38f);   // infinity counts as the largest finite value
     const float by = amax > 0.0f ? amax : 1.0f, qmax = f8_max(FMT);
-    // qmax / amax would overflow for the smallest maxima: those divide first
-    const bool small = by < 1.0e-30f;
-    const float mul = small ? qmax : __fdiv_rn(qmax, by);
-    if (small) {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-            v[j] = make_float4(__fdiv_rn(v[j].x, by), __fdiv_rn(v[j].y, by), __fdiv_rn(v[j].z, by), __fdiv_rn(v[j].w, by));
-    }
+    // qmax / amax would overflow for the smallest maxima: those blocks are raised first, which is exact
+    const float raise = by < 0x1p-100f ? 0x1p100f : 1.0f, mul = __fdiv_rn(qmax, by * raise);
+    const float below = mul * (1.0f - 0x1p-21f), above = mul * (1.0f + 0x1p-21f);
     if (threadIdx.x == 0) scales[blockIdx.x] = amax > 0.0f ? __fdiv_rn(amax, qmax) : 1.0f;
+    uint32_t open = 0;   // bit j: a code of v[j] is not settled
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
         const uint32_t r = bn * kBlock + warp + 16 * j;
         if (r >= N || c >= K) continue;
-        const uint32_t o = enc_f8x2(FMT, v[j].x * mul, v[j].y * mul) | enc_f8x2(FMT, v[j].z * mul, v[j].w * mul) << 16;
+        const float4 u = make_float4(v[j].x * raise, v[j].y * raise, v[j].z * raise, v[j].w * raise);
+        const uint32_t o = enc_f8x2(FMT, u.x * below, u.y * below) | enc_f8x2(FMT, u.z * below, u.w * below) << 16;
+        const uint32_t o1 = enc_f8x2(FMT, u.x * above, u.y * above) | enc_f8x2(FMT, u.z * above, u.w * above) << 16;
+        if (o != o1) open |= 1u << j;
         uint8_t *dst = q + (size_t)r * K + c;
         if (VEC) {
             *reinterpret_cast<uint32_t *>(dst) = o;
@@ -138,6 +153,11 @@ __global__ void __launch_bounds__(512, 2) quant_weights_kernel(const float *__re
             if (c + 2 < K) dst[2] = (uint8_t)(o >> 16);
             if (c + 3 < K) dst[3] = (uint8_t)(o >> 24);
         }
+    }
+    // the few open ones read their values again: kept until here they would cost the others registers
+    for (; open; open &= open - 1) {
+        const size_t at = (size_t)(bn * kBlock + warp + 16 * (__ffs(open) - 1)) * K + c;
+        for (uint32_t i = 0; i < 4 && c + i < K; ++i) q[at + i] = exact_f8<FMT>(w[at + i], by);
     }
 }
 
