@@ -17,6 +17,8 @@ namespace fp8 {
 
 constexpr uint32_t kBlock = 128;
 
+constexpr uint32_t blocks_of(uint32_t n) { return n / kBlock + (n % kBlock != 0); }   // of any n: no sum that wraps
+
 // 16 fp16 values a lane, 8 lanes a block: rows of H % 16 == 0 values, x 32-byte
 // and q 16-byte aligned. A block behind the row's end is short in its last lanes.
 template <int FMT>
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(512, 2) quant_weights_kernel(const float *__re
 cudaError_t launch_quantize_act_fp8(int fmt, const void *x, uint32_t T, uint32_t H, uint8_t *q, float *scales, cudaStream_t st)
 {
     using namespace fp8;
-    const uint32_t kb = (H + kBlock - 1) / kBlock;
+    const uint32_t kb = blocks_of(H);
     const uint64_t blocks = (uint64_t)T * kb;
     if (!blocks) return cudaSuccess;
     const bool wide = H % 16 == 0 && (reinterpret_cast<uintptr_t>(x) & 31u) == 0 && (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
@@ -183,7 +185,7 @@ cudaError_t launch_quantize_weights_fp8(int fmt, const float *w, uint32_t N, uin
 {
     using namespace fp8;
     if (!N || !K) return cudaSuccess;
-    const uint32_t kb = (K + kBlock - 1) / kBlock, nb = (N + kBlock - 1) / kBlock;
+    const uint32_t kb = blocks_of(K), nb = blocks_of(N);
     const bool vec = K % 4 == 0 && (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && (reinterpret_cast<uintptr_t>(q) & 3u) == 0;
     const unsigned grid = nb * kb;   // the caller keeps it below 2^31
     return launch_overlapped(vec ? (fmt == 1 ? quant_weights_kernel<1, true> : quant_weights_kernel<2, true>)
