@@ -210,8 +210,9 @@ __global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t *__rest
     }
 }
 
-// One CTA per token and 128 units of 16 bytes; slots summed in order, fp32. A thread has
-// eight rows' loads in flight: with one token that is the whole kernel.
+// One CTA per token and 128 units of 16 bytes (the grid's limit only makes it go on to
+// others); slots summed in order, fp32. A thread has eight rows' loads in flight: with one
+// token that is the whole kernel.
 constexpr int kCombineThreads = 128;
 
 template <bool F16>
@@ -220,30 +221,34 @@ __global__ void __launch_bounds__(kCombineThreads) combine_fp8_kernel(const floa
                                                                       const float4 *__restrict__ shared_y, void *__restrict__ out)
 {
     __shared__ int32_t rows[32];
-    const uint32_t t = blockIdx.x, c = blockIdx.y * kCombineThreads + threadIdx.x;
+    const uint32_t t = blockIdx.x;
     if (threadIdx.x < k) rows[threadIdx.x] = inv[(size_t)t * k + threadIdx.x];
+    uint32_t c = blockIdx.y * kCombineThreads + threadIdx.x;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (shared_y && c < units) acc = __ldcs(shared_y + (size_t)t * units + c);
     __syncthreads();
-    if (c >= units) return;
-    for (uint32_t j0 = 0; j0 < k; j0 += 8) {
-        float4 v[8];
+    while (c < units) {
+        for (uint32_t j0 = 0; j0 < k; j0 += 8) {
+            float4 v[8];
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-            const int32_t r = j0 + j < k ? rows[j0 + j] : -1;
-            v[j] = r >= 0 ? __ldcs(y + (size_t)r * units + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
+            for (uint32_t j = 0; j < 8; ++j) {
+                const int32_t r = j0 + j < k ? rows[j0 + j] : -1;
+                v[j] = r >= 0 ? __ldcs(y + (size_t)r * units + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-            acc.x += v[j].x;
-            acc.y += v[j].y;
-            acc.z += v[j].z;
-            acc.w += v[j].w;
+            for (uint32_t j = 0; j < 8; ++j) {
+                acc.x += v[j].x;
+                acc.y += v[j].y;
+                acc.z += v[j].z;
+                acc.w += v[j].w;
+            }
         }
+        const size_t at = (size_t)t * units + c;
+        if (F16) static_cast<uint2 *>(out)[at] = make_uint2(half2_bits(acc.x, acc.y), half2_bits(acc.z, acc.w));
+        else static_cast<float4 *>(out)[at] = acc;
+        c += gridDim.y * kCombineThreads;
+        acc = shared_y && c < units ? __ldcs(shared_y + (size_t)t * units + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    const size_t at = (size_t)t * units + c;
-    if (F16) static_cast<uint2 *>(out)[at] = make_uint2(half2_bits(acc.x, acc.y), half2_bits(acc.z, acc.w));
-    else static_cast<float4 *>(out)[at] = acc;
 }
 
 }  // namespace fp8
@@ -278,8 +283,8 @@ cudaError_t launch_fp8_scatter(int fmt, const int32_t *ids, const float *weights
 cudaError_t launch_fp8_combine(const float *y, const int32_t *inv, uint32_t T, uint32_t k, uint32_t H, const float *shared_y,
                                void *out, int f16, cudaStream_t st)
 {
-    const uint32_t units = H / 4;
-    const dim3 grid(T, (units + fp8::kCombineThreads - 1) / fp8::kCombineThreads);
+    const uint32_t units = H / 4, chunks = (units + fp8::kCombineThreads - 1) / fp8::kCombineThreads;
+    const dim3 grid(T, chunks < 65535 ? chunks : 65535);
     const float4 *a = reinterpret_cast<const float4 *>(y), *sy = reinterpret_cast<const float4 *>(shared_y);
     if (f16) fp8::combine_fp8_kernel<true><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, units, sy, out);
     else fp8::combine_fp8_kernel<false><<<grid, fp8::kCombineThreads, 0, st>>>(a, inv, k, units, sy, out);

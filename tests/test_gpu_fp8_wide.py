@@ -49,3 +49,31 @@ def test_quantize_weights_of_the_longest_side(ctx, rows, depth):
     assert not q[2:-3].any()
     want = np.float32([1, 2]) / np.float32(448)
     assert s[0].item() == want[0] and s[-1].item() == want[1] and (s[1:-1] == 1).all()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_layer_of_more_columns_than_the_grid_has(ctx, f16):
+    """Hidden size above 2^25: the rows' sums take more CTAs than one grid dimension has. One
+    expert and a shared one, whose mid is 448 in channel 0 and whose down weights are zero but
+    for a few columns at both ends and beside the limit."""
+    import mpp41
+    h, i, k = 2 ** 25 + 256, 128, 2
+    x = torch.zeros(1, h, dtype=torch.float16, device="cuda")
+    x[0, 0] = 448
+    one = int(F.to_fp8([1.0], "e4m3")[0])
+    zeros = lambda *s: torch.zeros(*s, dtype=torch.uint8, device="cuda")  # noqa: E731
+    wg, wu, wd = zeros(1, i, h), zeros(1, i, h), zeros(1, h, i)
+    wg[0, 0, 0] = wu[0, 0, 0] = one
+    at = torch.tensor([0, 1, 127, 2 ** 24, 2 ** 25 - 1, 2 ** 25, 2 ** 25 + 1, h - 1], device="cuda")
+    wd[0, at, 0] = one
+    sg, sd = torch.full((1, 1, h // 128), 2.0 ** -4, device="cuda"), torch.full((1, h // 128, 1), 2.0 ** -6, device="cuda")
+    # gate = up = 448 / 16 = 28: silu(28) * 28 = 784, and 784 / 64 = 12.25 from each of the three
+    d = mpp41.moe_fp8_desc(1, h, i, 1, k, shared_intermediate=i, out_f16=f16)
+    scratch = torch.empty(mpp41.moe_fp8_scratch_bytes(d), dtype=torch.uint8, device="cuda")
+    out = torch.full((1, h), 5.0, dtype=torch.float16 if f16 else torch.float32, device="cuda")
+    ctx.moe_fp8(d, x, torch.zeros(1, k, dtype=torch.int32, device="cuda"), torch.tensor([[1.0, -3.0]], device="cuda"), wg, sg, wu,
+                sg, wd, sd, out, scratch, shared=(wg, sg, wu, sg, wd, sd))
+    ctx.synchronize()
+    assert torch.all((out[0, at].double() + 12.25).abs() <= 12.25 * 2.0 ** -11 + 1e-5)
+    out[0, at] = 0
+    assert not out.any()
