@@ -30,7 +30,7 @@ __device__ __forceinline__ float amax_h(float amax) { return fminf(amax, 65504.0
 // midpoint of the 8-bit format (at most 5 significant bits) or is at least 2^-16
 // of its size away from one. The product with the rounded quotient qmax / amax is
 // within 2^-22; raising it by 0.7 * 2^-20 and cutting it to 20 significant bits
-// (quant16) puts it on the midpoint in the first case and leaves its side alone in
+// (snap) puts it on the midpoint in the first case and leaves its side alone in
 // the second, for one multiplication and one AND instead of a division a value.
 __device__ __forceinline__ void block_scale(float amax, float qmax, float &mul, float &scale)
 {

@@ -127,7 +127,8 @@ int launch_fp8_gemm(const Fp8Launch &L, cudaStream_t st, const char **why)
     // Pairs from 1024 rows a group: 4 to 5 % faster there (4096 x 14336 x 4096: 229 against
     // 238 us, 8192^3: 514 against 540), but their 256-row tiles round groups up further (32
     // groups of 512 rows on average: 287 against 265 us; a layer with 128 rows an expert:
-    // 439 against 370).
+    // 439 against 370). M counts a layer's every assignment, negative ids among them: a rank
+    // that holds few of the experts its ids name has fewer rows than this rule takes it to have.
     const uint64_t mt = L.offsets ? L.M / kBM + (L.groups < L.M ? L.groups : L.M) : (L.M + kBM - 1) / kBM;
     const uint64_t sms = (uint64_t)sm_count(dev);
     const bool few = !swiglu && !L.offsets && !more && mt * ((L.N + 255) / 256) < sms && mt * ((L.N + 127) / 128) <= sms;

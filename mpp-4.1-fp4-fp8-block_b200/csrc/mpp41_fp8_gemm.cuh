@@ -24,8 +24,8 @@
 // take it as long to issue as the block's MMAs take to run. Sixteen promotion warps of
 // half the columns (112 registers each) took 276 us.
 //
-// What bounds it: with many rows the promotion. That product takes 224 to 229 us
-// (2.1 PFLOP/s); of 244 us in an earlier form 48 went without the FMAs, 63 without reading
+// What bounds it: with many rows the promotion. That product takes 214 us (2.25 PFLOP/s)
+// in short runs, 247 at the power limit; of 244 us in an earlier form 48 went without the FMAs, 63 without reading
 // tensor memory either, 17 without the copies, and the epilogue's stores cost 20 of 230.
 // With few rows it is the stream of B from memory.
 #pragma once
